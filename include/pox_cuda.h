@@ -319,6 +319,107 @@ int pox_cuda_paged_attention(pox_cuda_ctx* ctx, const float* q_dev, const uint16
                              uint32_t head_dim, uint32_t num_blocks, uint32_t max_blocks_per_seq, float* out_dev,
                              void* stream);
 
+/* ---- 8-bit paged KV cache ------------------------------------------------------------------
+ * No counterpart in the reference (its KvCache is f32, engine.rs:10-84). Pages are of 16 tokens and
+ * addressed through block tables like the f16 pages above (paged_cache.rs:4,149-162). Every pointer
+ * below is device memory that the caller owns; calls are asynchronous on `stream` (a cudaStream_t;
+ * NULL = the context's stream, (void*)1 = the legacy default stream). */
+
+/* Rows of heads: element (row r, head h, dim d) at data[r * row_stride + h * head_stride + d], strides
+ * in elements. Row-major ([rows][heads][dim]), slices of a fused projection's rows and head-major
+ * buffers are all views of this kind. dtype POX_F32, POX_F16 or POX_BF16; data aligned to its element.
+ * Rows that are written must not overlap one another (POX_ERR_INVALID). Bases and strides that are
+ * multiples of 16 bytes take vector loads and stores, others go element by element. */
+typedef struct {
+    void* data;
+    int dtype;
+    uint64_t row_stride, head_stride;
+} pox_rows;
+
+/* Position rotation of the first rot_dim dims of a head: pair i turns by the angle whose (cos, sin) is
+ * table[position * rot_dim / 2 + i] (f32 pairs, `positions` rows of them). POX_ROPE_INTERLEAVED pairs
+ * dims (2 i, 2 i + 1) as the reference does (engine.rs:353-408), POX_ROPE_HALF pairs
+ * (i, i + rot_dim / 2). rot_dim is even, at most the head's dim; 0 = no rotation. */
+#define POX_ROPE_INTERLEAVED 0
+#define POX_ROPE_HALF 1
+typedef struct {
+    const float* table;
+    uint32_t positions, rot_dim;
+    int style;
+} pox_rope;
+
+/* Norms of queries and keys for each head, with the position rotation in the same pass:
+ *   y = x / sqrt(sum_d x_d^2 / head_dim + eps) * f16 norm_d, then rotated by rope at positions[row]
+ * in f32, rounded once to the rows' type. q_norm / k_norm [head_dim] may be NULL (that side is only
+ * rotated); heads or kv_heads 0 leaves that side out. All rows have one dtype; an output may be its own
+ * input (same data, same strides) and must not overlap it otherwise. head_dim is even, at most 512
+ * (else POX_ERR_UNSUPPORTED). A position outside the rotation table leaves its row unwritten and the
+ * next pox_cuda_synchronize returns POX_ERR_INVALID. */
+typedef struct {
+    pox_rows q, k, q_out, k_out;
+    uint32_t rows, heads, kv_heads, head_dim;
+    const uint16_t* q_norm;
+    const uint16_t* k_norm;
+    float eps;
+    pox_rope rope;
+    const uint32_t* positions; /* [rows]; may be NULL when rope.rot_dim is 0 */
+} pox_qk_norm_rope;
+int pox_cuda_qk_norm_rope(pox_cuda_ctx* ctx, const pox_qk_norm_rope* args, void* stream);
+
+/* The cache: pages [num_blocks][kv_heads][32 * head_dim] int8 and scales [num_blocks][kv_heads][2] f32
+ * (of k, of v): the value of an element is its byte times the scale of its page, head and side. Within
+ * a page of one kv head (hd = head_dim):
+ *   k of token t, dim d: byte t * hd + (d ^ 64 if hd == 128 and t is odd, else d)
+ *   v of token t, dim d: byte 16 * hd + 16 * d + t
+ * so that the attention's tensor-core operands are read from a page as it lies. head_dim 32, 64 or 128;
+ * pages 16-byte, scales 8-byte aligned. Contents need no initialisation: a page counts as empty until
+ * its slot 0 is written. */
+typedef struct {
+    int8_t* pages;
+    float* scales;
+    uint32_t num_blocks, kv_heads, head_dim;
+} pox_kv8_cache;
+
+/* New rows of `seqs` sequences, ragged: rows row_starts[s] .. row_starts[s + 1] belong to sequence s
+ * (row_starts [seqs + 1] ascends from 0 to `rows`; NULL = one row each). ctx_lens[s] counts the tokens of
+ * the sequence with its new rows: row i of n stands at position ctx_lens[s] - n + i, its page is
+ * block_tables[s * max_blocks_per_seq + position / 16]. A row whose position is negative is padding (a
+ * free slot of a fixed batch: ctx_lens[s] = 0). max_rows and max_ctx bound the rows and the context of
+ * any sequence (max_ctx <= 16 max_blocks_per_seq); they choose the launch. A sequence that breaks a
+ * bound, and pages outside [0, num_blocks), are left out on the device and the next
+ * pox_cuda_synchronize returns POX_ERR_INVALID. */
+typedef struct {
+    const uint32_t* row_starts;
+    const uint32_t* ctx_lens;
+    const int32_t* block_tables;
+    uint32_t seqs, rows, max_rows, max_ctx, max_blocks_per_seq;
+} pox_kv8_batch;
+
+/* Appends k and v (rows [batch->rows][kv_heads], one dtype; k rotated on the way unless rope is NULL or
+ * has rot_dim 0) at their positions. Scale rule, per page, kv head and side, in f32:
+ *   s' = max(s, max |x| / 127) over the rows that go to the page, s = 0 when slot 0 is among them;
+ *   a new element is stored as rint(x / s'), an element of an older slot as rint(byte * (s / s')).
+ * Older slots are the ones below the page's first new row; a page's scale never falls until its slot 0 is
+ * written again. Elements that are not finite do not enter the maximum: an infinity is stored as
+ * +-127, a NaN as 0. Two rows at one position in one call are not allowed. */
+int pox_cuda_kv8_append(pox_cuda_ctx* ctx, const pox_kv8_cache* cache, const pox_kv8_batch* batch, const pox_rows* k,
+                        const pox_rows* v, const pox_rope* rope, void* stream);
+/* Reads rows back: k and v (both rows [batch->rows][kv_heads], one dtype) receive byte * scale of the
+ * positions that batch names, padding rows 0. For exporting a prefix, for attention elsewhere, and to see
+ * what the cache holds. */
+int pox_cuda_kv8_read(pox_cuda_ctx* ctx, const pox_kv8_cache* cache, const pox_kv8_batch* batch, const pox_rows* k,
+                      const pox_rows* v, void* stream);
+/* Attention of the batch's rows over the cache, which already holds them (pox_cuda_kv8_append first):
+ *   out[r][h] = sum over t <= position(r) of p_t v_t, p = softmax_t(scale * q[r][h] . k_t)
+ * for query head h over kv head h / (heads / kv_heads); scale 0 = 1 / sqrt(head_dim). Softmax statistics
+ * and sums are f32; f16 and bf16 rows enter the products exactly, f32 rows as pairs of f16 (22
+ * bits); a row that sees nothing is 0. q and out: rows [batch->rows][heads] of one dtype. Sequences of few
+ * rows split their context over the GPU and are joined in the same launch, in a fixed order: results do
+ * not change from run to run. The first call on a stream, and one with larger sizes, allocates that
+ * stream's split partials (held by the context): make it before capturing the stream. */
+int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* cache, const pox_kv8_batch* batch, const pox_rows* q,
+                           const pox_rows* out, uint32_t heads, float scale, void* stream);
+
 /* ---- tensor-parallel decode across the GPUs of one node (one process and context per GPU) ----
  * The reference decodes on one device; the shard layout is the standard Megatron split, chosen so
  * that every .pox payload shards into contiguous row ranges or 128-aligned column ranges:

@@ -63,6 +63,44 @@ class LlamaConfig(C.Structure):
                 ("kv_heads", C.c_uint32), ("vocab", C.c_uint32), ("rms_eps", C.c_float), ("rope_theta", C.c_float)]
 
 
+class Rows(C.Structure):
+    """pox_rows: element (row r, head h, dim d) at data[r * row_stride + h * head_stride + d]."""
+
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("row_stride", C.c_uint64), ("head_stride", C.c_uint64)]
+
+
+POX_ROPE_INTERLEAVED, POX_ROPE_HALF = 0, 1
+
+
+class Rope(C.Structure):
+    """pox_rope: (cos, sin) pairs f32 [positions][rot_dim / 2] and how dims pair up."""
+
+    _fields_ = [("table", C.c_void_p), ("positions", C.c_uint32), ("rot_dim", C.c_uint32), ("style", C.c_int)]
+
+
+class QkNormRope(C.Structure):
+    """pox_qk_norm_rope: the arguments of CudaBackend.qk_norm_rope."""
+
+    _fields_ = [("q", Rows), ("k", Rows), ("q_out", Rows), ("k_out", Rows), ("rows", C.c_uint32),
+                ("heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("eps", C.c_float), ("rope", Rope), ("positions", C.c_void_p)]
+
+
+class Kv8Cache(C.Structure):
+    """pox_kv8_cache: int8 pages [num_blocks][kv_heads][32 * head_dim], scales [num_blocks][kv_heads][2]."""
+
+    _fields_ = [("pages", C.c_void_p), ("scales", C.c_void_p), ("num_blocks", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32)]
+
+
+class Kv8Batch(C.Structure):
+    """pox_kv8_batch: the new rows of a ragged batch of sequences and their block tables."""
+
+    _fields_ = [("row_starts", C.c_void_p), ("ctx_lens", C.c_void_p), ("block_tables", C.c_void_p),
+                ("seqs", C.c_uint32), ("rows", C.c_uint32), ("max_rows", C.c_uint32), ("max_ctx", C.c_uint32),
+                ("max_blocks_per_seq", C.c_uint32)]
+
+
 _lib = None
 
 
@@ -121,6 +159,13 @@ def _declare(L):
         "pox_cuda_model_buffers": (i32, [vp, C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(vp),
                                          C.POINTER(vp)]),
         "pox_cuda_paged_attention": (i32, [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, vp, vp]),
+        "pox_cuda_qk_norm_rope": (i32, [vp, C.POINTER(QkNormRope), vp]),
+        "pox_cuda_kv8_append": (i32, [vp, C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.POINTER(Rows), C.POINTER(Rows),
+                                      C.POINTER(Rope), vp]),
+        "pox_cuda_kv8_read": (i32, [vp, C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.POINTER(Rows), C.POINTER(Rows),
+                                    vp]),
+        "pox_cuda_kv8_attention": (i32, [vp, C.POINTER(Kv8Cache), C.POINTER(Kv8Batch), C.POINTER(Rows),
+                                         C.POINTER(Rows), u32, C.c_float, vp]),
         "pox_file_open": (i32, [C.c_char_p, C.POINTER(vp)]),
         "pox_file_from_bytes": (i32, [vp, sz, C.POINTER(vp)]),
         "pox_file_close": (None, [vp]),

@@ -189,3 +189,31 @@ class CudaBackend:
 
     def upload_f16(self, w_bits, rows, cols) -> ResidentTensor:
         return self.upload(L.POX_F16, rows, cols, w_bits)
+
+    # ---- 8-bit paged KV cache (device pointers in the structs of _lib.py; asynchronous on `stream`: a
+    # cudaStream_t, 0 = the context's stream, 1 = the legacy default stream) ------------------------------
+    def qk_norm_rope(self, args: L.QkNormRope, stream: int = 0) -> None:
+        """Per-head RMSNorm of q and k rows with the position rotation in the same pass."""
+        rc = L.lib().pox_cuda_qk_norm_rope(self.ctx, args, stream or None)
+        if rc:
+            L.check(rc)
+
+    def kv8_append(self, cache: L.Kv8Cache, batch: L.Kv8Batch, k: L.Rows, v: L.Rows, rope: Optional[L.Rope] = None,
+                   stream: int = 0) -> None:
+        """Appends k (rotated on the way) and v rows to the int8 pages at their sequences' positions."""
+        rc = L.lib().pox_cuda_kv8_append(self.ctx, cache, batch, k, v, rope, stream or None)
+        if rc:
+            L.check(rc)
+
+    def kv8_read(self, cache: L.Kv8Cache, batch: L.Kv8Batch, k: L.Rows, v: L.Rows, stream: int = 0) -> None:
+        """Reads the values of the batch's positions back into k and v rows."""
+        rc = L.lib().pox_cuda_kv8_read(self.ctx, cache, batch, k, v, stream or None)
+        if rc:
+            L.check(rc)
+
+    def kv8_attention(self, cache: L.Kv8Cache, batch: L.Kv8Batch, q: L.Rows, out: L.Rows, heads: int,
+                      scale: float = 0.0, stream: int = 0) -> None:
+        """Causal attention of the batch's q rows over the int8 pages (scale 0: 1 / sqrt(head_dim))."""
+        rc = L.lib().pox_cuda_kv8_attention(self.ctx, cache, batch, q, out, heads, scale, stream or None)
+        if rc:
+            L.check(rc)

@@ -21,7 +21,9 @@ enum { kErrWaitRing = 1, kErrWaitX = 2, kErrWaitEnt = 4 };  // bits of the kerne
 enum { kErrPersist = 256 };  // the persistent decode kernel: a grid-barrier or ring wait expired
 // Bits for invalid input found on the device (reported as POX_ERR_INVALID rather than a timeout): a
 // decode position at or beyond 16 x max_blocks_per_seq, a block-table entry outside [0, kv_blocks).
-enum { kErrAttnPos = 64, kErrAttnPage = 128, kErrInputMask = kErrAttnPos | kErrAttnPage };
+// 8-bit cache: a position outside the rotation table, a sequence that breaks its batch's bounds.
+enum { kErrAttnPos = 64, kErrAttnPage = 128, kErrRopePos = 512, kErrBatch = 1024,
+       kErrInputMask = kErrAttnPos | kErrAttnPage | kErrRopePos | kErrBatch };
 
 __host__ __device__ inline int kind_kblock(int kind) { return kind == kKindI4 ? 128 : (kind == kKindI8 ? 64 : 32); }
 

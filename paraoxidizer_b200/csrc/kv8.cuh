@@ -1,0 +1,115 @@
+// kv8.cuh -- what the kernels of the 8-bit paged KV cache share: the page layout, views of rows, the
+// ragged batch and the rotation, as include/pox_cuda.h describes them.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "gemv.cuh"
+#include "model.h"
+
+namespace pox {
+
+// Byte of (token t, dim d) within the page of one kv head. K rows of 128 dims swap their 64-byte halves
+// at odd tokens: a warp's 16-byte reads of two neighbouring tokens then cover all 32 banks.
+template <int HD>
+__host__ __device__ __forceinline__ constexpr int kv8_k_off(int t, int d) {
+    return t * HD + (HD == 128 ? d ^ ((t & 1) << 6) : d);
+}
+template <int HD>
+__host__ __device__ __forceinline__ constexpr int kv8_v_off(int t, int d) {
+    return kPage * HD + d * kPage + t;
+}
+
+struct Kv8Cache {
+    int8_t* pages;
+    float* scales;
+    uint32_t num_blocks;
+    int kvh;
+};
+
+struct Kv8Batch {
+    const uint32_t* row_starts;  // NULL: one row each
+    const uint32_t* ctx_lens;
+    const int32_t* btab;
+    uint32_t seqs, rows, max_rows, max_ctx, mbps;
+};
+
+template <typename T>
+struct RowsView {
+    T* data;
+    size_t row, head;  // strides in elements
+    __device__ __forceinline__ T* at(size_t r, size_t h) const { return data + r * row + h * head; }
+};
+
+struct RopeView {
+    const float2* table;  // [positions][rot / 2]
+    uint32_t positions;
+    int rot;   // 0: none
+    int half;  // pairs (i, i + rot / 2), else (2 i, 2 i + 1)
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) {
+    return x;
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) {
+    return __float2half_rn(x);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+    return __float2bfloat16_rn(x);
+}
+
+// One pair turned by (cos, sin): separate products and sums, so that the result does not depend on
+// which kernel contracts them (the quantised bytes are then the same everywhere).
+__device__ __forceinline__ float2 rope_turn(float a, float b, float2 cs) {
+    return make_float2(__fsub_rn(__fmul_rn(a, cs.x), __fmul_rn(b, cs.y)),
+                       __fadd_rn(__fmul_rn(a, cs.y), __fmul_rn(b, cs.x)));
+}
+
+// Rows, context and first row of sequence s; false (reported) if it breaks the batch's bounds.
+struct SeqSpan {
+    uint32_t r0;
+    int n, ctx;
+};
+__device__ __forceinline__ bool seq_span(const Kv8Batch& b, uint32_t s, SeqSpan& o, int* err) {
+    const uint32_t r0 = b.row_starts ? b.row_starts[s] : s, r1 = b.row_starts ? b.row_starts[s + 1] : s + 1;
+    const uint32_t ctx = b.ctx_lens[s];
+    o.r0 = r0, o.n = (int)(r1 - r0), o.ctx = (int)ctx;
+    if (r1 < r0 || r1 > b.rows || r1 - r0 > b.max_rows || ctx > b.max_ctx) {
+        if ((threadIdx.x & 31) == 0) atomicOr(err, kErrBatch);
+        return false;
+    }
+    return true;
+}
+
+// The sequence of item i when sequence s owns the items f(row_starts[s], s) .. f(row_starts[s + 1], s + 1) with
+// f(x, s) = (x + per_seq * s) / div: the largest s with f <= i (a bound of the items, f ascends with row_starts). Whole warp:
+// 32 candidates a round, so two dependent loads serve 1024 sequences.
+__device__ __forceinline__ uint32_t find_seq(const Kv8Batch& b, uint32_t i, uint32_t per_seq, uint32_t div) {
+    if (!b.row_starts) return min(((unsigned long long)i * div) / (per_seq + 1), (unsigned long long)b.seqs - 1);
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t lo = 0, n = b.seqs;  // the answer is in [lo, lo + n)
+    while (n > 1) {
+        const uint32_t step = (n + 31) / 32;
+        const uint32_t s = lo + lane * step;
+        const bool le = lane * step < n && ((unsigned long long)b.row_starts[s] + (unsigned long long)per_seq * s) / div <= i;
+        const unsigned m = __ballot_sync(0xffffffffu, le);
+        const uint32_t k = m ? 31 - __clz(m) : 0;
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    return lo;
+}
+
+}  // namespace pox

@@ -155,9 +155,11 @@ int pox::take_kernel_error(pox_cuda_ctx* ctx) {
     if (f == 0) return POX_OK;
     *(volatile int*)ctx->err_host = 0;
     if ((f & ~kErrInputMask) == 0)
-        return set_error(POX_ERR_INVALID, "attention input rejected on the device (flag 0x%x:%s%s); results of that call "
+        return set_error(POX_ERR_INVALID, "attention input rejected on the device (flag 0x%x:%s%s%s%s); results of that call "
                          "are invalid", f, (f & kErrAttnPos) ? " a position beyond its block table" : "",
-                         (f & kErrAttnPage) ? " a block-table entry outside [0, kv_blocks)" : "");
+                         (f & kErrAttnPage) ? " a block-table entry outside [0, kv_blocks)" : "",
+                         (f & kErrRopePos) ? " a position outside the rotation table" : "",
+                         (f & kErrBatch) ? " a sequence beyond its batch's bounds" : "");
     return set_error(POX_ERR_TIMEOUT, "a kernel's bounded wait expired (flag 0x%x); results of that call are invalid", f);
 }
 
