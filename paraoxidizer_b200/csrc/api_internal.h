@@ -42,6 +42,17 @@ struct pox_tensor {
     size_t h_outlier_len = 0;
 };
 
+namespace pox {
+// What the attention over the 8-bit cache keeps for each stream that calls it (calls on different
+// streams may overlap): split partials, and one ticket per item, zero between launches.
+struct Kv8Scratch {
+    float* part = nullptr;
+    size_t part_bytes = 0;
+    uint32_t* tickets = nullptr;
+    size_t items = 0;
+};
+}  // namespace pox
+
 struct pox_cuda_ctx {
     int device = 0;
     int num_sms = 148;
@@ -68,6 +79,7 @@ struct pox_cuda_ctx {
     size_t tc_tickets_n = 0;
     void* attn_scratch = nullptr;  // kernel-level paged attention: split partials
     size_t attn_scratch_bytes = 0;
+    std::unordered_map<cudaStream_t, pox::Kv8Scratch> kv8;
     int* err_host = nullptr;  // kernel error flag (host-mapped); nonzero = a bounded wait expired or bad input
     int* err_dev = nullptr;
     std::vector<pox_model*> models;  // decode models created on this context (destroyed with it)

@@ -243,6 +243,39 @@ static Kv8Batch batch_view(const pox_kv8_batch* b) {
                     b->max_blocks_per_seq};
 }
 
+// The stream's split partials and tickets for a plan that splits.
+static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, uint32_t hd, Kv8StepPlan& p) {
+    if (p.splits <= 1) return POX_OK;
+    const size_t need = p.items * p.splits * (p.pair ? 8 : 16) * (hd + 2) * sizeof(float);
+    try {
+        std::lock_guard<std::mutex> lk(ctx->mu);
+        Kv8Scratch& k = ctx->kv8[st];
+        if (need > k.part_bytes || p.items > k.items) {
+            cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+            if (cudaStreamIsCapturing(st, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone)
+                return set_error(POX_ERR_INVALID, "split partials must be sized by a call before stream capture");
+            cudaError_t e = cudaStreamSynchronize(st);  // earlier calls may still use the old ones
+            if (e != cudaSuccess) return cuda_error(e, "cudaStreamSynchronize");
+            const size_t bytes = std::max(need, k.part_bytes), items = std::max(p.items, k.items);
+            cudaFree(k.part);
+            cudaFree(k.tickets);
+            k = Kv8Scratch();
+            e = cudaMalloc(&k.part, bytes);
+            if (e == cudaSuccess) k.part_bytes = bytes, e = cudaMalloc(&k.tickets, items * sizeof(uint32_t));
+            if (e == cudaSuccess) k.items = items, e = cudaMemsetAsync(k.tickets, 0, items * sizeof(uint32_t), st);
+            if (e != cudaSuccess) {
+                k.items = 0;  // so that the next call allocates and clears again
+                return cuda_error(e, "split partials");
+            }
+        }
+        p.part = k.part;
+        p.tickets = k.tickets;
+    } catch (const std::exception& x) {  // (no exception crosses the C boundary)
+        return set_error(POX_ERR_OOM, "split partials: %s", x.what());
+    }
+    return POX_OK;
+}
+
 template <typename T>
 static cudaError_t launch_qk(pox_cuda_ctx* ctx, const pox_qk_norm_rope* a, cudaStream_t st) {
     QkArgs<T> k;
@@ -387,11 +420,20 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     cudaError_t e = cudaSetDevice(ctx->device);
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
+    const int G = (int)(heads / c->kv_heads), es = esize(q->dtype);
+    Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, G, q->dtype == POX_F32, ctx->num_sms);
+    if (plan.items * (unsigned __int128)plan.splits > 0x7fffffffu)
+        return set_error(POX_ERR_UNSUPPORTED, "%zu items of %d splits", plan.items, plan.splits);
+    plan.device = ctx->device;
+    rc = kv8_scratch(ctx, st, c->head_dim, plan);
+    if (rc) return rc;
+    const int vec = (((uintptr_t)q->data | (uintptr_t)out->data) % (4 * es)) == 0 &&
+                    ((q->row_stride | q->head_stride | out->row_stride | out->head_stride) % 4) == 0;
     e = by_shape(c->head_dim, q->dtype, [&](auto hd, auto t) {
         using T = decltype(t);
-        Kv8Attn<T> a{cache_view(c), batch_view(b), rows_view<const T>(*q), rows_view<T>(*out), (int)(heads / c->kv_heads),
-                     scale > 0.f ? scale : 1.0f / sqrtf((float)c->head_dim), ctx->err_dev};
-        return launch_kv8_attention<decltype(hd)::value, T>(a, st);
+        const float s = (scale > 0.f ? scale : 1.0f / sqrtf((float)c->head_dim)) * 1.4426950408889634f;
+        Kv8Attn<T> a{cache_view(c), batch_view(b), rows_view<const T>(*q), rows_view<T>(*out), G, s, vec, ctx->err_dev};
+        return launch_kv8_step<decltype(hd)::value, T>(a, plan, st);
     });
     return e == cudaSuccess ? POX_OK : cuda_error(e, "kv8_attention launch");
 }
