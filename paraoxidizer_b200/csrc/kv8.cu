@@ -243,6 +243,8 @@ static Kv8Batch batch_view(const pox_kv8_batch* b) {
                     b->max_blocks_per_seq};
 }
 
+constexpr int kPromptRows = 64;
+
 // The stream's split partials and tickets for a plan that splits.
 static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, uint32_t hd, Kv8StepPlan& p) {
     if (p.splits <= 1) return POX_OK;
@@ -421,11 +423,17 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
     const int G = (int)(heads / c->kv_heads), es = esize(q->dtype);
-    Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, G, q->dtype == POX_F32, ctx->num_sms);
+    // Sequences of more rows than kPromptRows go to the tensor-memory kernel; a batch may hold both kinds,
+    // told apart on the device. All rows equal (or one sequence) means one kind.
+    const long long most = (long long)b->max_rows * G;
+    const bool prompt = c->head_dim != 32 && q->dtype != POX_F32 && most > kPromptRows;
+    const bool step = !prompt || (b->seqs > 1 && b->rows != (unsigned long long)b->seqs * b->max_rows);
+    Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, G, q->dtype == POX_F32, ctx->num_sms,
+                                     prompt ? kPromptRows : 0x7fffffff);
     if (plan.items * (unsigned __int128)plan.splits > 0x7fffffffu)
         return set_error(POX_ERR_UNSUPPORTED, "%zu items of %d splits", plan.items, plan.splits);
     plan.device = ctx->device;
-    rc = kv8_scratch(ctx, st, c->head_dim, plan);
+    rc = step ? kv8_scratch(ctx, st, c->head_dim, plan) : POX_OK;
     if (rc) return rc;
     const int vec = (((uintptr_t)q->data | (uintptr_t)out->data) % (4 * es)) == 0 &&
                     ((q->row_stride | q->head_stride | out->row_stride | out->head_stride) % 4) == 0;
@@ -433,7 +441,12 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
         using T = decltype(t);
         const float s = (scale > 0.f ? scale : 1.0f / sqrtf((float)c->head_dim)) * 1.4426950408889634f;
         Kv8Attn<T> a{cache_view(c), batch_view(b), rows_view<const T>(*q), rows_view<T>(*out), G, s, vec, ctx->err_dev};
-        return launch_kv8_step<decltype(hd)::value, T>(a, plan, st);
+        constexpr int HD = decltype(hd)::value;
+        cudaError_t r = cudaSuccess;
+        if constexpr (HD != 32 && sizeof(T) == 2)
+            if (prompt) r = launch_kv8_prompt<HD, T>(a, kPromptRows + 1, ctx->device, st);
+        if (r == cudaSuccess && step) r = launch_kv8_step<HD, T>(a, plan, st);
+        return r;
     });
     return e == cudaSuccess ? POX_OK : cuda_error(e, "kv8_attention launch");
 }

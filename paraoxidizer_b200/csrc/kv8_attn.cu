@@ -6,54 +6,9 @@
 // where k_t and v_t are the stored whole numbers. Taking the maximum over u instead of s puts the scale of
 // v into the exponent: the products see whole numbers and p <= 2^8, and no page's scale multiplies a tile.
 #include "kv8_attn.h"
+#include "kv8_math.cuh"
 
 namespace pox {
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
-
-// Power of two that brings a row whose largest magnitude is m to [2^13, 2^14): f16 then holds bf16 values
-// exactly and an f32 value's two terms to 22 bits; values below 2^-27 m lose bits, which are 2^-38 m.
-__device__ __forceinline__ float row_factor(float m, float& inverse) {
-    int e = (int)((__float_as_uint(m) >> 23) & 255) - 127;
-    e = m > 0.f && m < INFINITY ? max(e, -100) : 13;
-    inverse = __uint_as_float((uint32_t)(127 + e - 13) << 23);
-    return __uint_as_float((uint32_t)(127 + 13 - e) << 23);
-}
-
-template <typename T>
-__device__ __forceinline__ void load4(const T* x, int vec, float (&v)[4]) {
-    if (vec) {
-        T t[4];
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(x);
-        else *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(x);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = to_f32(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = to_f32(x[i]);
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void store4(T* x, int vec, float4 v) {
-    if (vec) {
-        T t[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(t);
-        else *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(t);
-    } else {
-        x[0] = from_f32<T>(v.x), x[1] = from_f32<T>(v.y), x[2] = from_f32<T>(v.z), x[3] = from_f32<T>(v.w);
-    }
-}
 
 constexpr int kStepStages = 4;  // pages in flight per warp
 
@@ -83,7 +38,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, 3) kv8_attn_step_kernel(Kv8At
     SeqSpan sq;
     if (!seq_span(a.b, s, sq, a.err)) return;
     const int rows = sq.n * a.G, row0 = rt * RT;
-    if (row0 >= rows) return;
+    if (row0 >= rows || rows > p.most_rows) return;
     const int pos0 = sq.ctx - sq.n, pmin = pos0 + row0 / a.G, pmax = pos0 + (min(row0 + RT, rows) - 1) / a.G;
     const int pages = pmax < 0 ? 0 : pmax / kPage + 1;
     const int ns = max(1, (pages + p.pages_per_split - 1) / p.pages_per_split);

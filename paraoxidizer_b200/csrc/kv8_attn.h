@@ -31,13 +31,15 @@ struct Kv8StepPlan {
     uint32_t* tickets = nullptr;  // [items], zero between launches
     size_t items = 0;
     int device = 0;
+    int most_rows = 0x7fffffff;  // sequences of more rows are left to the prompt kernel
     bool pair = true;  // 8 rows a tile, each as two f16 terms; else 16 rows
 };
 
 // Rows of a tile: f32 rows, and any rows that fit 8, are carried as pairs of f16 terms.
-inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int G, bool f32, int sms) {
+inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int G, bool f32, int sms, int most_rows) {
     Kv8StepPlan p;
-    const long long rows = (long long)b.max_rows * G;
+    p.most_rows = most_rows;
+    const long long rows = std::min((long long)b.max_rows * G, (long long)most_rows);
     p.pair = f32 || rows <= 8;
     const int rt = p.pair ? 8 : 16;
     p.row_tiles = (int)((rows + rt - 1) / rt);
@@ -62,7 +64,11 @@ inline cudaError_t kv8_smem_once(F* kernel, int bytes, int device, std::atomic<u
     return e;
 }
 
+// Sequences of at most p.most_rows rows (tokens times query heads of the group), any head dim.
 template <int HD, typename T>
 cudaError_t launch_kv8_step(const Kv8Attn<T>& a, const Kv8StepPlan& p, cudaStream_t st);
+// Sequences of at least min_rows rows, head dims 64 and 128, f16 and bf16.
+template <int HD, typename T>
+cudaError_t launch_kv8_prompt(const Kv8Attn<T>& a, int min_rows, int device, cudaStream_t st);
 
 }  // namespace pox

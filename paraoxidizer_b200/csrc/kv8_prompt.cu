@@ -1,0 +1,378 @@
+// kv8_prompt.cu -- attention of many rows (prompts and prompt chunks) over int8 pages on the 5th-generation
+// tensor cores.
+//
+// The same mathematics as kv8_attn.cu: u_t = scale log2(e) a q . k_t + log2 b, p_t = 2^(u_t - m),
+// out = sum p_t v_t / sum p_t / b with whole numbers k_t, v_t and page scales a, b. The rows of a kv head are its
+// (token, query head of the group) pairs in order, 128 to a tile; causal masking is by each row's own position.
+#include "kv8_attn.h"
+#include "kv8_math.cuh"
+#include "tc05.cuh"
+
+namespace pox {
+
+// D[tmem] (+)= A[tmem] * B[smem]^T: A is M = 128 lanes of packed f16 pairs, 8 columns for 16 k.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+constexpr int kPromptKeys = 128;                   // tokens of a tile: 8 pages
+constexpr int kPromptThreads = 32 * (4 + 4 + 4 + 1);  // two softmax warpgroups, the converters, the MMA warp
+
+template <int HD>
+struct PromptSmem {
+    static constexpr int kQ = 128 * HD * 2;             // bytes of one q tile
+    static constexpr int kHalf = kPromptKeys * HD * 2;  // K or V of a tile in f16
+    static constexpr int kStages = 4;                   // two tiles of each
+    static constexpr int total = 2 * kQ + kStages * kHalf;
+};
+
+// One CTA per (sequence, kv head, 256 rows): two tiles of 128 rows share every K and V tile. Warps 0-3 and 4-7
+// hold the softmax of one tile each (a thread a row), warps 8-11 turn int8 pages into f16 operand tiles
+// (exactly) in the 128-byte-swizzled K-major layout, one thread of warp 12 issues the products:
+//   S = Q K^T (shared x shared -> TMEM), O += P V (P packed f16 in TMEM over S's columns, V shared).
+// While one tile's softmax runs, the tensor core works on the other's products. The reference m of a row moves only when p
+// would pass 2^8 (then its warp rescales O in TMEM), so that O is hardly ever read before the end. p is rounded to
+// f16 (2^-11 of p, as f16 and bf16 outputs are rounded to no more), the sums of p and O are f32. f32 rows stay with the
+// step kernel: carried as two f16 terms through these products, an output was 7e-6 off (the tensor core drops low bits
+// as it adds up) where mma.sync is 3e-7 off.
+// An MMA completes in order with those issued before it: S of tile j ready means P V of tile j - 1 done.
+template <int HD, typename T>
+__global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8Attn<T> a, int min_rows) {
+    using SM = PromptSmem<HD>;
+    constexpr int NST = SM::kStages, QB = SM::kQ, HB = SM::kHalf;
+    constexpr uint32_t TS = 0, TO = 256;  // TMEM columns: S of tile t at 128 t, O at 256 + HD t
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * NST + 5];
+    __shared__ uint32_t tmem_base;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * NST, sfull = empty + 8 * NST, pready = sfull + 16,
+                   ofull = pready + 16;
+
+    // long tiles first: the last rows of a sequence see the most tokens
+    const uint32_t pairs = a.b.seqs * (uint32_t)a.c.kvh, tiles = gridDim.x / pairs;
+    const uint32_t h = blockIdx.x % a.c.kvh, s = blockIdx.x / a.c.kvh % a.b.seqs;
+    const int tile = (int)(tiles - 1 - blockIdx.x / pairs);
+    SeqSpan sq;
+    if (!seq_span(a.b, s, sq, a.err)) return;
+    const int rows = sq.n * a.G, row0 = tile * 256;
+    if (rows < min_rows || row0 >= rows) return;
+    const int pos0 = sq.ctx - sq.n, pmax = pos0 + (min(row0 + 256, rows) - 1) / a.G;
+    const int nt = row0 + 128 < rows ? 2 : 1, nk = pmax < 0 ? 0 : pmax / kPromptKeys + 1;
+    const int32_t* bt = a.b.btab + (size_t)s * a.b.mbps;
+    const int last_page = pmax < 0 ? -1 : pmax / kPage;
+
+    if (warp == 12) {
+        if (lane == 0) {
+            for (int i = 0; i < NST; i++) mbar_init(full + 8 * i, 4), mbar_init(empty + 8 * i, 1);
+            for (int i = 0; i < 2; i++) mbar_init(sfull + 8 * i, 1), mbar_init(pready + 8 * i, 4);
+            mbar_init(ofull, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        tmem_alloc(smem_u32(&tmem_base), 512);
+        tmem_relinquish();
+    }
+    const uint32_t qs = smem, kv = smem + 2 * QB;
+
+    // q rows to f16 operand tiles (a thread a row), scaled by a power of two per row
+    const int ti = warp >> 2, row = row0 + tid;  // softmax warps: the row of tile ti that this thread keeps
+    const bool mine = tid < 256 && row < rows;
+    float qf = 0.f;
+    if (tid < 128 * nt) {
+        const T* q = a.q.at((size_t)sq.r0 + (mine ? row / a.G : 0), h * a.G + (mine ? row % a.G : 0));
+        float f = 1.f, inv = 1.f;
+        if constexpr (!std::is_same<T, __half>::value) {
+            float m = 0.f;
+#pragma unroll 4
+            for (int d = 0; d < HD; d += 4) {
+                float v[4];
+                load4(q + d, a.vec, v);
+                m = fmaxf(fmaxf(m, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+            }
+            f = row_factor(m, inv);
+        }
+        qf = inv * a.scale;
+        const uint32_t r = tid & 127, qt = qs + ti * QB;
+#pragma unroll 4
+        for (int d = 0; d < HD; d += 8) {
+            float v[8];
+            load4(q + d, a.vec, *reinterpret_cast<float(*)[4]>(v));
+            load4(q + d + 4, a.vec, *reinterpret_cast<float(*)[4]>(v + 4));
+            uint32_t x[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = mine ? pack_f16(v[2 * i] * f, v[2 * i + 1] * f) : 0u;
+            sts128(qt + (d / 64) * (128 * 128) + sw128_off(r, (d % 64) / 8), x[0], x[1], x[2], x[3]);
+        }
+        fence_proxy_async_smem();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tm = tmem_base;
+    bool bad = false;
+
+    if (warp < 8) {  // ---- softmax of tile ti
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tm + TS + 128 * ti + lanes,
+                       to = tm + TO + HD * ti + lanes;
+        const int rpos = mine ? pos0 + row / a.G : 0x3fffffff;
+        const int wpos = pos0 + (row0 + 32 * warp) / a.G;  // the first row of the warp sees no further
+        float m = -INFINITY, l = 0.f;
+        if (ti < nt) {
+            // lane i < 8 looks after page i of a tile: its entry two tiles ahead, its scales one tile ahead
+            auto entry = [&](int j) {
+                const int page = 8 * j + lane;
+                return lane < 8 && page <= last_page ? bt[page] : -1;
+            };
+            auto scales = [&](int blk, int j) {
+                if (blk < 0 || (uint32_t)blk >= a.c.num_blocks) {  // left out: u is -inf whatever S
+                    if (lane < 8 && 8 * j + lane <= last_page) atomicOr(a.err, kErrAttnPage);
+                    return make_float2(0.f, -1.f);
+                }
+                return *reinterpret_cast<const float2*>(a.c.scales + ((size_t)blk * a.c.kvh + h) * 2);
+            };
+            float2 ab = scales(entry(0), 0);
+            int next = entry(1);
+            for (int j = 0; j < nk; j++) {
+                const float lb = ab.y == -1.f ? -INFINITY : log2f(fmaxf(ab.y, 1e-30f) + (ab.y - ab.y)),
+                            ib = ab.y == -1.f ? 0.f : 1.0f / fmaxf(ab.y, 1e-30f), ka = ab.x;
+                if (j + 1 < nk) ab = scales(next, j + 1), next = entry(j + 2);
+                if (!bad) bad = __any_sync(0xffffffffu, !mbar_wait(sfull + 8 * ti, j & 1));
+                if (bad) break;
+                tc_fence_after();
+                const bool cut = j * kPromptKeys + kPromptKeys - 1 > wpos;
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    float x[32];
+                    tmem_ld32(ts + 32 * c, x);
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        const float f = qf * __shfl_sync(0xffffffffu, ka, 2 * c + g),
+                                    pl = __shfl_sync(0xffffffffu, lb, 2 * c + g);
+                        float y = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            float z = x[16 * g + i];
+                            if (cut && j * kPromptKeys + 32 * c + 16 * g + i > rpos) z = -INFINITY;
+                            y = fmaxf(y, z);
+                        }
+                        mx = fmaxf(mx, fmaf(y, f, pl));
+                    }
+                }
+                if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
+                    const float go = mx > m + 8.0f ? mx : m;
+                    const float f = m == -INFINITY ? (go == -INFINITY ? 1.f : 0.f) : ex2(m - go);
+                    m = go;
+                    l *= f;
+                    if (j) {
+#pragma unroll
+                        for (int c = 0; c < HD / 32; c++) {
+                            float x[32];
+                            tmem_ld32(to + 32 * c, x);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) x[i] *= f;
+                            tmem_st32(to + 32 * c, x);
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    float x[32];
+                    tmem_ld32(ts + 32 * c, x);
+                    uint32_t hi[16];
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        const float f = qf * __shfl_sync(0xffffffffu, ka, 2 * c + g),
+                                    pl = __shfl_sync(0xffffffffu, lb, 2 * c + g) - ref,
+                                    pi = __shfl_sync(0xffffffffu, ib, 2 * c + g);
+                        float sum = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            float z = fmaf(x[16 * g + i], f, pl);
+                            if (cut && j * kPromptKeys + 32 * c + 16 * g + i > rpos) z = -INFINITY;
+                            x[16 * g + i] = ex2(z);
+                            sum += x[16 * g + i];
+                        }
+                        if (sum != 0.f) l = fmaf(sum, pi, l);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; i++) hi[i] = pack_f16(x[2 * i], x[2 * i + 1]);
+                    tmem_st16(ts + 16 * c, hi);  // over columns of S that have been read
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(pready + 8 * ti);
+            }
+            if (nk && !bad) bad = __any_sync(0xffffffffu, !mbar_wait(ofull, 0));
+            tc_fence_after();
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            T* y = a.out.at((size_t)sq.r0 + (mine ? row / a.G : 0), h * a.G + (mine ? row % a.G : 0));
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) {
+                float x[32];
+                if (nk) tmem_ld32(to + 32 * c, x);
+                else
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = 0.f;
+                if (mine && !bad)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        store4(y + 32 * c + i, a.vec,
+                               make_float4(x[i] * inv, x[i + 1] * inv, x[i + 2] * inv, x[i + 3] * inv));
+            }
+        }
+    } else if (warp < 12) {  // ---- converters: pages 2 w and 2 w + 1 of each tile
+        const int w = warp - 8, b = lane & 7, g = lane >> 3;
+        constexpr int NI = HD / 16;  // 16-byte pieces of K (or V) per lane and tile
+        uint4 kr[NI], vr[NI];
+        auto page_at = [&](int j, int i) -> const int8_t* {
+            const int page = 8 * j + 2 * w + i, blk = page <= last_page ? bt[page] : -1;
+            return blk >= 0 && (uint32_t)blk < a.c.num_blocks ? a.c.pages + ((size_t)blk * a.c.kvh + h) * (32 * HD)
+                                                              : nullptr;
+        };
+        auto load_k = [&](const int8_t* p0, const int8_t* p1) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int8_t* p = i < NI / 2 ? p0 : p1;
+                const int q = i % (NI / 2), t = 8 * (q & 1) + b, c = 4 * (q >> 1) + g;
+                kr[i] = p ? ldg128_nc(p + kv8_k_off<HD>(t, 16 * c)) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto load_v = [&](const int8_t* p0, const int8_t* p1) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int8_t* p = i < NI / 2 ? p0 : p1;
+                vr[i] = p ? ldg128_nc(p + kv8_v_off<HD>(0, 32 * (i % (NI / 2)) + 8 * g + b)) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto put = [&](uint32_t at0, uint32_t at1, uint4 x) {
+            uint32_t r[8];
+            i8x4_to_f16x4(x.x, r[0], r[1]);
+            i8x4_to_f16x4(x.y, r[2], r[3]);
+            i8x4_to_f16x4(x.z, r[4], r[5]);
+            i8x4_to_f16x4(x.w, r[6], r[7]);
+            sts128(at0, r[0], r[1], r[2], r[3]);
+            sts128(at1, r[4], r[5], r[6], r[7]);
+        };
+        auto ready = [&](int st) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * st);
+        };
+        const int8_t *p0 = page_at(0, 0), *p1 = page_at(0, 1);
+        if (nk) load_k(p0, p1);
+        for (int j = 0; j < nk; j++) {
+            load_v(p0, p1);
+            if (j + 1 < nk) p0 = page_at(j + 1, 0), p1 = page_at(j + 1, 1);
+            int n = 2 * j, st = n % NST;
+            if (n >= NST) bad = __any_sync(0xffffffffu, !mbar_wait(empty + 8 * st, (n / NST - 1) & 1));
+            if (bad) break;
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int q = i % (NI / 2), t = 16 * (2 * w + i / (NI / 2)) + 8 * (q & 1) + b, c = 4 * (q >> 1) + g;
+                const uint32_t base = kv + st * HB + (c / 4) * (kPromptKeys * 128);
+                put(base + sw128_off(t, 2 * (c % 4)), base + sw128_off(t, 2 * (c % 4) + 1), kr[i]);
+            }
+            ready(st);
+            if (j + 1 < nk) load_k(p0, p1);
+            n++, st = n % NST;
+            if (n >= NST) bad = __any_sync(0xffffffffu, !mbar_wait(empty + 8 * st, (n / NST - 1) & 1));
+            if (bad) break;
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int page = 2 * w + i / (NI / 2), d = 32 * (i % (NI / 2)) + 8 * g + b;
+                const uint32_t base = kv + st * HB + (page / 4) * (HD * 128);
+                put(base + sw128_off(d, 2 * (page % 4)), base + sw128_off(d, 2 * (page % 4) + 1), vr[i]);
+            }
+            ready(st);
+        }
+    } else if (lane == 0 && nk) {  // ---- the products
+        constexpr uint32_t is = umma_idesc_f16(128, kPromptKeys), ip = umma_idesc_f16(128, HD);
+        auto wait_full = [&](int n) {
+            if (!bad) bad = !mbar_wait(full + 8 * (n % NST), (n / NST) & 1);
+            tc_fence_after();
+        };
+        auto scores = [&](int t, int j) {
+            const uint32_t k0 = kv + (2 * j % NST) * HB;
+#pragma unroll
+            for (int k = 0; k < HD / 16; k++)
+                umma_f16(tm + TS + 128 * t, umma_desc_sw128(qs + t * QB + (k / 4) * (128 * 128)) + 2 * (k % 4),
+                         umma_desc_sw128(k0 + (k / 4) * (kPromptKeys * 128)) + 2 * (k % 4), is, k);
+            umma_commit(sfull + 8 * t);
+        };
+        auto values = [&](int t, int j) {
+            if (!bad) bad = !mbar_wait(pready + 8 * t, j & 1);
+            tc_fence_after();
+            if (bad) return;
+            const uint32_t v0 = kv + ((2 * j + 1) % NST) * HB;
+#pragma unroll
+            for (int k = 0; k < kPromptKeys / 16; k++)
+                umma_f16_ts(tm + TO + HD * t, tm + TS + 128 * t + 8 * k,
+                            umma_desc_sw128(v0 + (k / 4) * (HD * 128)) + 2 * (k % 4), ip, j || k);
+        };
+        wait_full(0);
+        if (!bad) {
+            for (int t = 0; t < nt; t++) scores(t, 0);
+            umma_commit(empty);
+        }
+        for (int j = 0; j < nk && !bad; j++) {
+            wait_full(2 * j + 1);
+            for (int t = 0; t < nt && !bad; t++) {
+                values(t, j);
+                if (t == nt - 1) umma_commit(empty + 8 * ((2 * j + 1) % NST));
+                if (j + 1 < nk) {
+                    if (t == 0) wait_full(2 * j + 2);
+                    if (!bad) scores(t, j + 1);
+                    if (t == nt - 1) umma_commit(empty + 8 * ((2 * j + 2) % NST));
+                }
+            }
+        }
+        umma_commit(ofull);
+        if (bad) mbar_wait(ofull, 0);  // what was issued ends before the tensor memory is given back
+    }
+    if (bad && lane == 0) atomicOr(a.err, kErrWaitRing);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tm, 512);
+    }
+}
+
+template <int HD, typename T>
+cudaError_t launch_kv8_prompt(const Kv8Attn<T>& a, int min_rows, int device, cudaStream_t st) {
+    constexpr int smem = PromptSmem<HD>::total + 1024;
+    static_assert(smem + 1024 <= 227 * 1024, "shared memory of a CTA");
+    static std::atomic<uint32_t> done{0};
+    const cudaError_t e = kv8_smem_once(&kv8_attn_prompt_kernel<HD, T>, smem, device, done);
+    if (e != cudaSuccess) return e;
+    const unsigned long long tiles = ((unsigned long long)a.b.max_rows * a.G + 255) / 256;
+    kv8_attn_prompt_kernel<HD, T><<<(unsigned)(tiles * a.b.seqs * a.c.kvh), kPromptThreads, smem, st>>>(a, min_rows);
+    return cudaGetLastError();
+}
+
+#define POX_KV8_PROMPT(HD)                                                                                  \
+    template cudaError_t launch_kv8_prompt<HD, __half>(const Kv8Attn<__half>&, int, int, cudaStream_t);     \
+    template cudaError_t launch_kv8_prompt<HD, __nv_bfloat16>(const Kv8Attn<__nv_bfloat16>&, int, int, cudaStream_t);
+POX_KV8_PROMPT(64)
+POX_KV8_PROMPT(128)
+
+}  // namespace pox
