@@ -8,6 +8,7 @@
 #include "api_internal.h"
 #include "kv8.cuh"
 #include "kv8_attn.h"
+#include "kv8_math.cuh"
 
 namespace pox {
 
@@ -25,9 +26,9 @@ struct QkArgs {
     int* err;
 };
 
-// One warp per (row, head): a pass for the sum of squares, one for the pairs.
+// Any shape: one warp per (row, head), a pass for the sum of squares and one for the pairs.
 template <typename T>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs<T> a) {
+__global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(QkArgs<T> a) {
     const int nh = a.heads[0] + a.heads[1], lane = threadIdx.x & 31;
     const unsigned long long item = (unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (item >= (unsigned long long)a.rows * nh) return;
@@ -63,6 +64,107 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs<T> a) {
     for (int d = rot + lane; d < a.hd; d += 32) y[d] = from_f32<T>(val(d));
 }
 
+// Bound by HBM (each element once in, once out), by the launch for a few rows. 16 bytes a load: of the L = hd / (2 V)
+// lanes of a head (V elements in 16 bytes), lane c holds the V dims from c V and the V dims from rot / 2 + c V, so that both
+// kinds of pairs lie within a lane, and what is not rotated in order behind. A warp takes 32 / L heads of a row at once and
+// `steps` such groups of it, two in flight, and keeps the row's (cos, sin) meanwhile.
+template <typename T, int L>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs<T> a, int steps, int groups) {
+    constexpr int V = 16 / sizeof(T), HW = 32 / L;
+    const int lane = threadIdx.x & 31, c = lane % L, nh = a.heads[0] + a.heads[1], rot = a.rope.rot;
+    const unsigned long long item = (unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const uint32_t r = (uint32_t)(item / groups);
+    if (r >= a.rows) return;
+    const int h0 = (int)(item % groups) * steps * HW + lane / L, turn = c < rot / (2 * V);
+    const int d0 = turn ? c * V : 2 * c * V, d1 = turn ? rot / 2 + c * V : d0 + V;
+    const uint32_t p = rot ? a.pos[r] : 0;
+    if (rot && p >= a.rope.positions) {
+        if (lane == 0) atomicOr(a.err, kErrRopePos);
+        return;
+    }
+    // the pair index of element i of the lower piece (and, interleaved, of the upper one)
+    __align__(16) float2 cs[V];
+    if (turn) {
+        const float4* t = reinterpret_cast<const float4*>(a.rope.table + (size_t)p * (rot / 2));
+        float4* q = reinterpret_cast<float4*>(cs);
+#pragma unroll
+        for (int i = 0; i < V / 2; i++)
+            q[i] = __ldg(t + (a.rope.half ? c * V / 2 + i : i < V / 4 ? c * V / 4 + i : (rot / 2 + c * V) / 4 + i - V / 4));
+    }
+    const T* src[2];
+    T* dst[2];
+    uint4 x[2][2];
+    auto fetch = [&](int k, int i) {
+        const int h = h0 + k * HW, side = h >= a.heads[0];
+        if (k < steps && h < nh) {
+            src[i] = a.in[side].at(r, h - (side ? a.heads[0] : 0));
+            dst[i] = a.out[side].at(r, h - (side ? a.heads[0] : 0));
+            x[i][0] = *reinterpret_cast<const uint4*>(src[i] + d0);
+            x[i][1] = *reinterpret_cast<const uint4*>(src[i] + d1);
+        }
+    };
+    auto finish = [&](int k, int i) {
+        const int h = h0 + k * HW, side = h >= a.heads[0];
+        const bool live = k < steps && h < nh;
+        float v[2][V];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int e = 0; e < V; e++) v[u][e] = live ? to_f32(reinterpret_cast<const T*>(&x[i][u])[e]) : 0.f;
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; e++) ss = fmaf(v[0][e], v[0][e], fmaf(v[1][e], v[1][e], ss));
+#pragma unroll
+        for (int o = L / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (!live) return;
+        const __half* w = a.w[side];
+        if (w) {
+            const float inv = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
+            __align__(16) __half g[2][V];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const __half* q = w + (u ? d1 : d0);
+                if constexpr (V == 8) *reinterpret_cast<uint4*>(g[u]) = __ldg(reinterpret_cast<const uint4*>(q));
+                else *reinterpret_cast<uint2*>(g[u]) = __ldg(reinterpret_cast<const uint2*>(q));
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int e = 0; e < V; e++) v[u][e] = v[u][e] * inv * __half2float(g[u][e]);
+        }
+        if (turn) {
+            if (a.rope.half) {
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const float2 y = rope_turn(v[0][e], v[1][e], cs[e]);
+                    v[0][e] = y.x, v[1][e] = y.y;
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        const float2 y = rope_turn(v[u][e], v[u][e + 1], cs[u * (V / 2) + e / 2]);
+                        v[u][e] = y.x, v[u][e + 1] = y.y;
+                    }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            __align__(16) T t[V];
+#pragma unroll
+            for (int e = 0; e < V; e++) t[e] = from_f32<T>(v[u][e]);
+            *reinterpret_cast<uint4*>(dst[i] + (u ? d1 : d0)) = *reinterpret_cast<const uint4*>(t);
+        }
+    };
+    for (int k = 0; k < steps; k += 2) {
+        fetch(k, 0);
+        fetch(k + 1, 1);
+        finish(k, 0);
+        finish(k + 1, 1);
+    }
+}
+
 // ---- append ----------------------------------------------------------------------------------------
 template <typename T>
 struct AppendArgs {
@@ -76,95 +178,247 @@ struct AppendArgs {
 // A page of the batch: sequence s owns page items (row_starts[s] + 30 s) / 16 .. (a bound of the pages that
 // its n rows touch: n rows reach at most (n + 30) / 16 pages, in closed form, so no scan over the sequences).
 __device__ __forceinline__ uint32_t page_base(const Kv8Batch& b, uint32_t s) {
-    return b.max_rows == 1 && !b.row_starts ? s : (uint32_t)(((unsigned long long)b.row_starts[s] + 30ull * s) / 16);
+    return !b.row_starts ? s : (uint32_t)(((unsigned long long)b.row_starts[s] + 30ull * s) / 16);
 }
 
-// One warp per (touched page, kv head, side): the page's new rows set the scale, its older slots follow.
-template <int HD, typename T>
-__global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32_t items) {
-    const int lane = threadIdx.x & 31, E = HD / 32;
-    const unsigned long long u = (unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const uint32_t item = (uint32_t)(u / (2 * a.c.kvh));
-    const int side = (int)(u % 2), h = (int)(u / 2 % a.c.kvh);
-    if (item >= items) return;
-    const uint32_t s = a.b.row_starts ? find_seq(a.b, item, 30, 16) : item;
+// What a unit of the append and read kernels works on: one page of one kv head, k or v, by a group of HD / 4
+// lanes, lane c of it on dims 4 c .. 4 c + 3 of all 16 tokens.
+struct PageUnit {
     SeqSpan sp;
-    if (!seq_span(a.b, s, sp, a.err)) return;
-    const int p0 = max(sp.ctx - sp.n, 0), page = p0 / kPage + (int)(item - page_base(a.b, s));
-    if (sp.ctx <= p0 || page * kPage >= sp.ctx) return;
-    const int first = max(p0 - page * kPage, 0), last = min(sp.ctx - page * kPage, kPage);
-    const int blk = a.b.btab[(size_t)s * a.b.mbps + page];
-    if (blk < 0 || (uint32_t)blk >= a.c.num_blocks) {
-        if (lane == 0) atomicOr(a.err, kErrAttnPage);
-        return;
+    int page, first, last;  // its slots first .. last - 1 are rows of the batch
+    size_t row;             // the row of slot `first`
+    int8_t* bytes;          // the page of the kv head
+    float* scale;
+};
+template <int HD>
+__device__ __forceinline__ bool page_unit(const Kv8Cache& c, const Kv8Batch& b, uint32_t item, int h, int side, PageUnit& o,
+                                          int* err) {
+    const uint32_t s = b.row_starts ? find_seq<HD / 4>(b, item, 30, 16) : item;
+    if (!seq_span(b, s, o.sp, err)) return false;
+    const int begin = o.sp.ctx - o.sp.n, p0 = max(begin, 0);
+    const int j = (int)(item - page_base(b, s));
+    if (j < 0) {  // row_starts does not begin at 0
+        if ((threadIdx.x & (HD / 4 - 1)) == 0) atomicOr(err, kErrBatch);
+        return false;
     }
-    const int rot = a.rope.rot, half = rot / 2;
-    if (side == 0 && rot && (uint32_t)(page * kPage + last - 1) >= a.rope.positions) {
-        if (lane == 0) atomicOr(a.err, kErrRopePos);
-        return;
+    o.page = p0 / kPage + j;
+    o.first = max(p0 - o.page * kPage, 0), o.last = min(o.sp.ctx - o.page * kPage, kPage);
+    o.row = (size_t)o.sp.r0 + (o.page * kPage + o.first - begin);
+    o.bytes = nullptr;
+    if (o.sp.ctx <= p0 || o.page * kPage >= o.sp.ctx) return true;
+    const int blk = b.btab[(size_t)s * b.mbps + o.page];
+    if (blk < 0 || (uint32_t)blk >= c.num_blocks) {
+        if ((threadIdx.x & (HD / 4 - 1)) == 0) atomicOr(err, kErrAttnPage);
+        return false;
     }
-    int8_t* pg = a.c.pages + ((size_t)blk * a.c.kvh + h) * (2 * kPage * HD);
-    float* sc = a.c.scales + ((size_t)blk * a.c.kvh + h) * 2 + side;
-    auto elem = [&](int t, int d) {  // the row element that slot t stores
-        const int pos = page * kPage + t;
-        const T* x = a.x[side].at((size_t)sp.r0 + (pos - (sp.ctx - sp.n)), h);
-        float v = to_f32(x[d]);
-        if (side == 0 && d < rot) {
-            const bool low = a.rope.half ? d < half : !(d & 1);
-            const int o = a.rope.half ? (low ? d + half : d - half) : d ^ 1, i = a.rope.half ? (low ? d : o) : d / 2;
-            const float w = to_f32(x[o]);
-            const float2 r = rope_turn(low ? v : w, low ? w : v, a.rope.table[(size_t)pos * half + i]);
-            v = low ? r.x : r.y;
+    o.bytes = c.pages + ((size_t)blk * c.kvh + h) * (2 * kPage * HD);
+    o.scale = c.scales + ((size_t)blk * c.kvh + h) * 2 + side;
+    return true;
+}
+
+// rint(x / s) as a byte: the quotient by Markstein's method (a correctly rounded reciprocal, one residual), the rounding by
+// adding 1.5 * 2^23, whose sum's low byte is the two's complement of the whole number.
+__device__ __forceinline__ uint32_t quantise(float x, float s, float rs) {
+    const float y = __fmul_rn(x, rs);
+    return __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-y, s, x), rs, y), 12582912.0f));
+}
+__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return prmt(prmt(a, b, 0x0040), prmt(c, d, 0x0040), 0x5410);
+}
+
+// Bound by HBM: rows in once, bytes out once. The page's new rows set the scale (a maximum over the group's lanes), its
+// older slots follow if the scale grew. All rows of a page are in flight at once; a lane's four dims make a word of each K
+// row and 64 contiguous bytes of V.
+template <int HD, typename T>
+__global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32_t items, int vec) {
+    constexpr int L = HD / 4, UW = 32 / L;
+    const int lane = threadIdx.x & 31, c = lane % L;
+    const unsigned long long u = ((unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * UW + lane / L;
+    const uint32_t item = min((uint32_t)(u / (2 * a.c.kvh)), items - 1);
+    const int h = (int)(u % a.c.kvh), side = (int)(u / a.c.kvh % 2);
+    PageUnit o;
+    bool live = u < (unsigned long long)items * 2 * a.c.kvh;
+    live = page_unit<HD>(a.c, a.b, item, h, side, o, a.err) && live && o.bytes;
+    const int rot = side ? 0 : a.rope.rot, half = rot / 2, pos0 = o.page * kPage;
+    if (live && rot && (uint32_t)(pos0 + o.last - 1) >= a.rope.positions) {
+        if (c == 0) atomicOr(a.err, kErrRopePos);
+        live = false;
+    }
+    const int first = live ? o.first : 0, last = live ? o.last : 0;
+    float v[kPage][4];
+    const float old = live && first ? *o.scale : 0.f;
+    uint4 ov[4];  // older bytes of V (a lane's dims), where the page is not written whole
+    const bool whole = first == 0 && last == kPage;
+    if (live && side && !whole)
+#pragma unroll
+        for (int e = 0; e < 4; e++) ov[e] = *reinterpret_cast<const uint4*>(o.bytes + kv8_v_off<HD>(0, 4 * c + e));
+    const T* x = a.x[side].at(live ? o.row : 0, h);
+#pragma unroll
+    for (int t = 0; t < kPage; t++) {
+        if (t >= first && t < last) load4(x + (size_t)(t - first) * a.x[side].row + 4 * c, vec, v[t]);
+        else v[t][0] = v[t][1] = v[t][2] = v[t][3] = 0.f;
+    }
+    if (__any_sync(0xffffffffu, rot > 0)) {
+        const bool mine = 4 * c < rot, by_lane = a.rope.half && a.rope.rot % 8 == 0, odd = a.rope.half && !by_lane;
+        const int step = rot / 8, from = 4 * c < half ? lane + step : lane - step;
+#pragma unroll
+        for (int t = 0; t < kPage; t++) {
+            if (!__any_sync(0xffffffffu, t >= first && t < last)) continue;
+            const float2* tab = a.rope.table + (size_t)(t >= first && t < last ? pos0 + t : 0) * half;
+            const bool on = mine && t >= first && t < last;
+            if (!odd) {
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = by_lane ? __shfl_sync(0xffffffffu, v[t][e], mine ? from : lane) : 0.f;
+                if (on && by_lane) {
+                    const int i = 4 * c < half ? 4 * c : 4 * c - half;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float2 cs = __ldg(tab + i + e);
+                        const float2 y = 4 * c < half ? rope_turn(v[t][e], w[e], cs) : rope_turn(w[e], v[t][e], cs);
+                        v[t][e] = 4 * c < half ? y.x : y.y;
+                    }
+                } else if (on) {
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2)
+                        if (4 * c + e < rot) {
+                            const float2 y = rope_turn(v[t][e], v[t][e + 1], __ldg(tab + 2 * c + e / 2));
+                            v[t][e] = y.x, v[t][e + 1] = y.y;
+                        }
+                }
+            } else if (on) {  // halves that do not fall on whole lanes: the partner from memory
+                const T* xr = x + (size_t)(t - first) * a.x[side].row;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int d = 4 * c + e;
+                    if (d < half) v[t][e] = rope_turn(v[t][e], to_f32(xr[d + half]), tab[d]).x;
+                    else if (d < rot) v[t][e] = rope_turn(to_f32(xr[d - half]), v[t][e], tab[d - half]).y;
+                }
+            }
         }
-        return v;
+    }
+    // the largest magnitude by its bits: what is not finite shows as the largest of all
+    uint32_t m = 0;
+#pragma unroll
+    for (int t = 0; t < kPage; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(v[t][e]) & 0x7fffffffu);
+#pragma unroll
+    for (int k = L / 2; k; k >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
+    if (__any_sync(0xffffffffu, m >= 0x7f800000u)) {  // rare: infinities saturate, NaN is 0, neither sets the scale
+        m = 0;
+#pragma unroll
+        for (int t = 0; t < kPage; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (fabsf(v[t][e]) < INFINITY) m = max(m, __float_as_uint(v[t][e]) & 0x7fffffffu);
+#pragma unroll
+        for (int k = L / 2; k; k >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
+        const float now = fmaxf(old, __fdiv_rn(__uint_as_float(m), 127.f));
+#pragma unroll
+        for (int t = 0; t < kPage; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[t][e] = v[t][e] == v[t][e] ? fminf(fmaxf(v[t][e], -127.f * now), 127.f * now) : 0.f;
+    }
+    if (!live) return;
+    const float now = fmaxf(old, __fdiv_rn(__uint_as_float(m), 127.f));
+    const bool grew = first && now > old;
+    const float ratio = grew ? __fdiv_rn(old, now) : 1.f;
+    // a scale so small that its reciprocal overflows or is not exact enough: both sides times 2^64
+    const float up = now < 0x1p-100f ? 0x1p64f : 1.f, s = now > 0.f ? now * up : 1.f, rs = __frcp_rn(s);
+    auto older = [&](uint32_t w, int n) {  // the first n bytes of a word to the new scale
+        uint32_t q[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            q[e] = e < n ? __float_as_uint(__fadd_rn(__fmul_rn((float)(int8_t)(w >> 8 * e), ratio), 12582912.0f))
+                         : w >> 8 * e;
+        return pack_bytes(q[0], q[1], q[2], q[3]);
     };
-    float m = 0.f;
-    for (int t = first; t < last; t++)
-        for (int e = 0; e < E; e++) {
-            const float v = fabsf(elem(t, lane + 32 * e));
-            if (v < INFINITY) m = fmaxf(m, v);  // false for NaN too
-        }
-    m = warp_max(m);
-    const float old = first ? *sc : 0.f;
-    const float now = fmaxf(old, __fdiv_rn(m, 127.f));
-    const float ratio = now > 0.f ? __fdiv_rn(old, now) : 0.f;
-    auto put = [&](int t, int d) -> int8_t& { return pg[side ? kv8_v_off<HD>(t, d) : kv8_k_off<HD>(t, d)]; };
-    for (int e = 0; e < E; e++) {
-        const int d = lane + 32 * e;
-        for (int t = 0; t < first; t++) put(t, d) = (int8_t)__float2int_rn(__fmul_rn((float)put(t, d), ratio));
-        for (int t = first; t < last; t++) {
-            const float q = now > 0.f ? __fdiv_rn(elem(t, d), now) : 0.f;
-            put(t, d) = (int8_t)__float2int_rn(fminf(fmaxf(q, -127.f), 127.f) * (q == q ? 1.f : 0.f));
+    if (side == 0) {
+        if (grew)
+            for (int t = 0; t < first; t++) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(o.bytes + kv8_k_off<HD>(t, 4 * c));
+                *w = older(*w, 4);
+            }
+#pragma unroll
+        for (int t = 0; t < kPage; t++)
+            if (t >= first && t < last) {
+                uint32_t q[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) q[e] = quantise(v[t][e] * up, s, rs);
+                *reinterpret_cast<uint32_t*>(o.bytes + kv8_k_off<HD>(t, 4 * c)) = pack_bytes(q[0], q[1], q[2], q[3]);
+            }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t b = whole ? 0u : k == 0 ? ov[e].x : k == 1 ? ov[e].y : k == 2 ? ov[e].z : ov[e].w;
+                uint32_t q[4];
+#pragma unroll
+                for (int t = 0; t < 4; t++) q[t] = quantise(v[4 * k + t][e] * up, s, rs);
+                w[k] = pack_bytes(q[0], q[1], q[2], q[3]);
+                if (!whole) {
+                    const uint32_t keep = grew ? older(b, first - 4 * k) : b;
+                    uint32_t mask = 0;  // bytes of slots first .. last - 1
+#pragma unroll
+                    for (int t = 0; t < 4; t++) mask |= 4 * k + t >= first && 4 * k + t < last ? 0xffu << 8 * t : 0u;
+                    w[k] = (w[k] & mask) | (keep & ~mask);
+                }
+            }
+            *reinterpret_cast<uint4*>(o.bytes + kv8_v_off<HD>(0, 4 * c + e)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
-    __syncwarp();
-    if (lane == 0) *sc = now;
+    if (c == 0) *o.scale = now;
 }
 
 // ---- reading rows back -------------------------------------------------------------------------------
+// The append's units the other way round. The unit of a sequence's first page also clears its padding rows.
 template <int HD, typename T>
-__global__ void __launch_bounds__(128) kv8_read_kernel(Kv8Cache c, Kv8Batch b, RowsView<T> k, RowsView<T> v, int* err) {
-    const int lane = threadIdx.x & 31;
-    const unsigned long long u = (unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const uint32_t r = (uint32_t)(u / c.kvh);
-    const int h = (int)(u % c.kvh);
-    if (r >= b.rows) return;
-    const uint32_t s = b.row_starts ? find_seq(b, r, 0, 1) : r;
-    SeqSpan sp;
-    if (!seq_span(b, s, sp, err)) return;
-    const int pos = sp.ctx - sp.n + (int)(r - sp.r0);
-    const int blk = pos >= 0 ? b.btab[(size_t)s * b.mbps + pos / kPage] : 0;
-    if (blk < 0 || (uint32_t)blk >= c.num_blocks) {
-        if (lane == 0) atomicOr(err, kErrAttnPage);
-        return;
+__global__ void __launch_bounds__(128) kv8_read_kernel(Kv8Cache cache, Kv8Batch b, RowsView<T> k, RowsView<T> v,
+                                                       uint32_t items, int vec, int* err) {
+    constexpr int L = HD / 4, UW = 32 / L;
+    const int lane = threadIdx.x & 31, c = lane % L;
+    const unsigned long long u = ((unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * UW + lane / L;
+    const uint32_t item = min((uint32_t)(u / (2 * cache.kvh)), items - 1);
+    const int h = (int)(u % cache.kvh), side = (int)(u / cache.kvh % 2);
+    PageUnit o;
+    const bool ok = page_unit<HD>(cache, b, item, h, side, o, err);
+    if (!ok || u >= (unsigned long long)items * 2 * cache.kvh) return;
+    const RowsView<T>& out = side ? v : k;
+    const int begin = o.sp.ctx - o.sp.n;
+    if (begin < 0 && o.page == 0)
+        for (int i = 0; i < min(-begin, o.sp.n); i++)
+            store4(out.at((size_t)o.sp.r0 + i, h) + 4 * c, vec, make_float4(0.f, 0.f, 0.f, 0.f));
+    if (!o.bytes) return;
+    const float s = *o.scale;
+    uint32_t w[kPage];  // K: the four dims of each token; V: four words of each dim
+    if (side == 0) {
+#pragma unroll
+        for (int t = 0; t < kPage; t++)
+            if (t >= o.first && t < o.last) w[t] = *reinterpret_cast<const uint32_t*>(o.bytes + kv8_k_off<HD>(t, 4 * c));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint4 x = *reinterpret_cast<const uint4*>(o.bytes + kv8_v_off<HD>(0, 4 * c + e));
+            w[4 * e] = x.x, w[4 * e + 1] = x.y, w[4 * e + 2] = x.z, w[4 * e + 3] = x.w;
+        }
     }
-    const int8_t* pg = c.pages + ((size_t)blk * c.kvh + h) * (2 * kPage * HD);
-    const float* sc = c.scales + ((size_t)blk * c.kvh + h) * 2;
-    const int t = pos % kPage;
-    for (int d = lane; d < HD; d += 32) {
-        k.at(r, h)[d] = from_f32<T>(pos < 0 ? 0.f : (float)pg[kv8_k_off<HD>(t, d)] * sc[0]);
-        v.at(r, h)[d] = from_f32<T>(pos < 0 ? 0.f : (float)pg[kv8_v_off<HD>(t, d)] * sc[1]);
-    }
+    T* y = out.at(o.row, h) + 4 * c;
+#pragma unroll
+    for (int t = 0; t < kPage; t++)
+        if (t >= o.first && t < o.last) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t q = side ? prmt(w[4 * e + t / 4], 0x4b000000u, 0x7440 + t % 4) : prmt(w[t], 0x4b000000u, 0x7440 + e);
+                // 2^23 + (byte + 128), exactly
+                x[e] = __fmul_rn(__uint_as_float(q ^ 0x80u) - 8388736.0f, s);
+            }
+            store4(y + (size_t)(t - o.first) * out.row, vec, make_float4(x[0], x[1], x[2], x[3]));
+        }
 }
 
 // ---- checks of arguments ------------------------------------------------------------------------------
@@ -288,9 +542,40 @@ static cudaError_t launch_qk(pox_cuda_ctx* ctx, const pox_qk_norm_rope* a, cudaS
     k.rows = a->rows, k.hd = (int)a->head_dim, k.eps = a->eps;
     k.rope = rope_view(&a->rope);
     k.pos = a->positions, k.err = ctx->err_dev;
-    const unsigned long long items = (unsigned long long)a->rows * (a->heads + a->kv_heads);
-    qk_norm_rope_kernel<T><<<(unsigned)((items + 7) / 8), 256, 0, st>>>(k);
+    const int V = 16 / (int)sizeof(T), hd = (int)a->head_dim, L = hd / (2 * V), nh = (int)(a->heads + a->kv_heads);
+    bool vec = hd % (2 * V) == 0 && k.rope.rot % (2 * V) == 0 && (L & (L - 1)) == 0 && L >= 2 && L <= 32 &&
+               ((uintptr_t)k.rope.table & 15) == 0;
+    for (int i = 0; i < 2; i++)
+        if (k.heads[i])
+            vec = vec && (((uintptr_t)k.in[i].data | (uintptr_t)k.out[i].data | (uintptr_t)k.w[i]) & 15) == 0 &&
+                  ((k.in[i].row | k.in[i].head | k.out[i].row | k.out[i].head) % V) == 0;
+    if (!vec) {
+        const unsigned long long items = (unsigned long long)a->rows * nh;
+        qk_norm_rope_any_kernel<T><<<(unsigned)((items + 7) / 8), 256, 0, st>>>(k);
+        return cudaGetLastError();
+    }
+    // as many groups of heads to a warp as leave every SM its 32 warps
+    const int all = (nh * L + 31) / 32;
+    const int steps = (int)std::min<long long>(std::max<long long>((long long)a->rows * all / (32LL * ctx->num_sms), 1),
+                                               std::min(all, 8));
+    const int groups = (all + steps - 1) / steps;
+    const unsigned grid = (unsigned)(((unsigned long long)a->rows * groups + 7) / 8);
+    switch (L) {
+        case 2: qk_norm_rope_kernel<T, 2><<<grid, 256, 0, st>>>(k, steps, groups); break;
+        case 4: qk_norm_rope_kernel<T, 4><<<grid, 256, 0, st>>>(k, steps, groups); break;
+        case 8: qk_norm_rope_kernel<T, 8><<<grid, 256, 0, st>>>(k, steps, groups); break;
+        case 16: qk_norm_rope_kernel<T, 16><<<grid, 256, 0, st>>>(k, steps, groups); break;
+        default: qk_norm_rope_kernel<T, 32><<<grid, 256, 0, st>>>(k, steps, groups);
+    }
     return cudaGetLastError();
+}
+
+static uint32_t page_items(const pox_kv8_batch* b) {
+    return b->row_starts ? (uint32_t)((b->rows + 30ull * b->seqs) / 16) : b->seqs;
+}
+// four elements of any (row, head) at once
+static int vec4(const pox_rows* r) {
+    return (uintptr_t)r->data % (4 * esize(r->dtype)) == 0 && (r->row_stride | r->head_stride) % 4 == 0;
 }
 
 template <int HD, typename T>
@@ -298,18 +583,19 @@ static cudaError_t launch_append(pox_cuda_ctx* ctx, const pox_kv8_cache* c, cons
                                  const pox_rows* v, const pox_rope* rope, cudaStream_t st) {
     AppendArgs<T> a{cache_view(c), batch_view(b), {rows_view<const T>(*k), rows_view<const T>(*v)}, rope_view(rope),
                     ctx->err_dev};
-    const uint32_t items = b->row_starts ? (uint32_t)((b->rows + 30ull * b->seqs) / 16 + 1) : b->seqs;
-    const unsigned long long warps = (unsigned long long)items * c->kv_heads * 2;
-    kv8_append_kernel<HD, T><<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(a, items);
+    const uint32_t items = page_items(b);
+    const unsigned long long lanes = (unsigned long long)items * c->kv_heads * 2 * (HD / 4);
+    kv8_append_kernel<HD, T><<<(unsigned)((lanes + 127) / 128), 128, 0, st>>>(a, items, vec4(k) && vec4(v));
     return cudaGetLastError();
 }
 
 template <int HD, typename T>
 static cudaError_t launch_read(pox_cuda_ctx* ctx, const pox_kv8_cache* c, const pox_kv8_batch* b, const pox_rows* k,
                                const pox_rows* v, cudaStream_t st) {
-    const unsigned long long warps = (unsigned long long)b->rows * c->kv_heads;
-    kv8_read_kernel<HD, T><<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(cache_view(c), batch_view(b), rows_view<T>(*k),
-                                                                        rows_view<T>(*v), ctx->err_dev);
+    const uint32_t items = page_items(b);
+    const unsigned long long lanes = (unsigned long long)items * c->kv_heads * 2 * (HD / 4);
+    kv8_read_kernel<HD, T><<<(unsigned)((lanes + 127) / 128), 128, 0, st>>>(
+        cache_view(c), batch_view(b), rows_view<T>(*k), rows_view<T>(*v), items, vec4(k) && vec4(v), ctx->err_dev);
     return cudaGetLastError();
 }
 
@@ -422,7 +708,7 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     cudaError_t e = cudaSetDevice(ctx->device);
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
-    const int G = (int)(heads / c->kv_heads), es = esize(q->dtype);
+    const int G = (int)(heads / c->kv_heads);
     // Sequences of more rows than kPromptRows go to the tensor-memory kernel; a batch may hold both kinds,
     // told apart on the device. All rows equal (or one sequence) means one kind.
     const long long most = (long long)b->max_rows * G;
@@ -435,8 +721,7 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     plan.device = ctx->device;
     rc = step ? kv8_scratch(ctx, st, c->head_dim, plan) : POX_OK;
     if (rc) return rc;
-    const int vec = (((uintptr_t)q->data | (uintptr_t)out->data) % (4 * es)) == 0 &&
-                    ((q->row_stride | q->head_stride | out->row_stride | out->head_stride) % 4) == 0;
+    const int vec = vec4(q) && vec4(out);
     e = by_shape(c->head_dim, q->dtype, [&](auto hd, auto t) {
         using T = decltype(t);
         const float s = (scale > 0.f ? scale : 1.0f / sqrtf((float)c->head_dim)) * 1.4426950408889634f;

@@ -93,18 +93,17 @@ __device__ __forceinline__ bool seq_span(const Kv8Batch& b, uint32_t s, SeqSpan&
     return true;
 }
 
-// The sequence of item i when sequence s owns the items f(row_starts[s], s) .. f(row_starts[s + 1], s + 1) with
-// f(x, s) = (x + per_seq * s) / div: the largest s with f <= i (a bound of the items, f ascends with row_starts). Whole warp:
-// 32 candidates a round, so two dependent loads serve 1024 sequences.
+// The sequence of item i when sequence s owns the items f(s) .. f(s + 1) - 1, f(s) = (row_starts[s] + per_seq s) / div:
+// the largest s with f(s) <= i. Called by whole warps, each group of W lanes with an item of its own: W candidates
+// a round, so two dependent loads serve 1024 sequences at W = 32.
+template <int W>
 __device__ __forceinline__ uint32_t find_seq(const Kv8Batch& b, uint32_t i, uint32_t per_seq, uint32_t div) {
-    if (!b.row_starts) return min(((unsigned long long)i * div) / (per_seq + 1), (unsigned long long)b.seqs - 1);
-    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t lane = threadIdx.x % W, shift = (threadIdx.x & 31) / W * W;
     uint32_t lo = 0, n = b.seqs;  // the answer is in [lo, lo + n)
-    while (n > 1) {
-        const uint32_t step = (n + 31) / 32;
-        const uint32_t s = lo + lane * step;
-        const bool le = lane * step < n && ((unsigned long long)b.row_starts[s] + (unsigned long long)per_seq * s) / div <= i;
-        const unsigned m = __ballot_sync(0xffffffffu, le);
+    while (__any_sync(0xffffffffu, n > 1)) {
+        const uint32_t step = (n + W - 1) / W, at = lane * step;
+        const bool le = at < n && ((unsigned long long)b.row_starts[lo + at] + (unsigned long long)per_seq * (lo + at)) / div <= i;
+        const uint32_t m = (__ballot_sync(0xffffffffu, le) >> shift) & (0xffffffffu >> (32 - W));
         const uint32_t k = m ? 31 - __clz(m) : 0;
         lo += k * step;
         n = min(step, n - k * step);
