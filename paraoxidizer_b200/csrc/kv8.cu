@@ -226,11 +226,15 @@ __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t 
     return prmt(prmt(a, b, 0x0040), prmt(c, d, 0x0040), 0x5410);
 }
 
+// How the append reads rows and turns k. kAny goes element by element and finds partners in memory; the others load
+// four elements at once and turn pairs within a lane (interleaved) or between lanes (halves of whole lanes).
+enum { kTurnAny = 0, kTurnNone = 1, kTurnHalf = 2, kTurnPairs = 3 };
+
 // Bound by HBM: rows in once, bytes out once. The page's new rows set the scale (a maximum over the group's lanes), its
 // older slots follow if the scale grew. All rows of a page are in flight at once; a lane's four dims make a word of each K
 // row and 64 contiguous bytes of V.
-template <int HD, typename T>
-__global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32_t items, int vec) {
+template <int HD, typename T, int TURN>
+__global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32_t items) {
     constexpr int L = HD / 4, UW = 32 / L;
     const int lane = threadIdx.x & 31, c = lane % L;
     const unsigned long long u = ((unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * UW + lane / L;
@@ -239,61 +243,87 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32
     PageUnit o;
     bool live = u < (unsigned long long)items * 2 * a.c.kvh;
     live = page_unit<HD>(a.c, a.b, item, h, side, o, a.err) && live && o.bytes;
-    const int rot = side ? 0 : a.rope.rot, half = rot / 2, pos0 = o.page * kPage;
+    const int rot = TURN == kTurnNone || side ? 0 : a.rope.rot, half = rot / 2, pos0 = o.page * kPage;
     if (live && rot && (uint32_t)(pos0 + o.last - 1) >= a.rope.positions) {
         if (c == 0) atomicOr(a.err, kErrRopePos);
         live = false;
     }
     const int first = live ? o.first : 0, last = live ? o.last : 0;
+    auto in = [&](int t) { return t >= first && t < last; };
+    const T* x = a.x[side].at(live ? o.row : 0, h);
+    const size_t ld = a.x[side].row;
     float v[kPage][4];
+    {
+        Raw4<T> raw[kPage];
+#pragma unroll
+        for (int t = 0; t < kPage; t++)
+            if (in(t)) raw[t].template load<TURN != kTurnAny>(x + (size_t)(t - first) * ld + 4 * c);
+#pragma unroll
+        for (int t = 0; t < kPage; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[t][e] = in(t) ? to_f32(raw[t].v[e]) : 0.f;
+    }
     const float old = live && first ? *o.scale : 0.f;
     uint4 ov[4];  // older bytes of V (a lane's dims), where the page is not written whole
     const bool whole = first == 0 && last == kPage;
     if (live && side && !whole)
 #pragma unroll
         for (int e = 0; e < 4; e++) ov[e] = *reinterpret_cast<const uint4*>(o.bytes + kv8_v_off<HD>(0, 4 * c + e));
-    const T* x = a.x[side].at(live ? o.row : 0, h);
+    if constexpr (TURN == kTurnHalf || TURN == kTurnPairs) {
+        const bool mine = 4 * c < rot, low = 4 * c < half;
+        const int from = !mine ? lane : low ? lane + rot / 8 : lane - rot / 8;
 #pragma unroll
-    for (int t = 0; t < kPage; t++) {
-        if (t >= first && t < last) load4(x + (size_t)(t - first) * a.x[side].row + 4 * c, vec, v[t]);
-        else v[t][0] = v[t][1] = v[t][2] = v[t][3] = 0.f;
-    }
-    if (__any_sync(0xffffffffu, rot > 0)) {
-        const bool mine = 4 * c < rot, by_lane = a.rope.half && a.rope.rot % 8 == 0, odd = a.rope.half && !by_lane;
-        const int step = rot / 8, from = 4 * c < half ? lane + step : lane - step;
+        for (int tc = 0; tc < kPage; tc += 4) {  // (cos, sin) of four rows in flight
+            if (!__any_sync(0xffffffffu, rot && last > tc && first < tc + 4)) continue;
+            float4 cs[4][2];
 #pragma unroll
-        for (int t = 0; t < kPage; t++) {
-            if (!__any_sync(0xffffffffu, t >= first && t < last)) continue;
-            const float2* tab = a.rope.table + (size_t)(t >= first && t < last ? pos0 + t : 0) * half;
-            const bool on = mine && t >= first && t < last;
-            if (!odd) {
-                float w[4];
+            for (int i = 0; i < 4; i++) {
+                const int t = tc + i;
+                if (mine && in(t)) {
+                    const float4* q = reinterpret_cast<const float4*>(a.rope.table + (size_t)(pos0 + t) * half +
+                                                                      (TURN == kTurnHalf ? 4 * c - (low ? 0 : half) : 2 * c));
+                    cs[i][0] = __ldg(q);
+                    if (TURN == kTurnHalf) cs[i][1] = __ldg(q + 1);
+                }
+            }
 #pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = by_lane ? __shfl_sync(0xffffffffu, v[t][e], mine ? from : lane) : 0.f;
-                if (on && by_lane) {
-                    const int i = 4 * c < half ? 4 * c : 4 * c - half;
+            for (int i = 0; i < 4; i++) {
+                const int t = tc + i;
+                const float2* q = reinterpret_cast<const float2*>(cs[i]);
+                if (TURN == kTurnHalf) {
+                    float w[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float2 cs = __ldg(tab + i + e);
-                        const float2 y = 4 * c < half ? rope_turn(v[t][e], w[e], cs) : rope_turn(w[e], v[t][e], cs);
-                        v[t][e] = 4 * c < half ? y.x : y.y;
+                    for (int e = 0; e < 4; e++) w[e] = __shfl_sync(0xffffffffu, v[t][e], from);
+                    if (mine && in(t))
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            v[t][e] = low ? rope_turn(v[t][e], w[e], q[e]).x : rope_turn(w[e], v[t][e], q[e]).y;
+                } else if (mine && in(t)) {
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float2 y = rope_turn(v[t][e], v[t][e + 1], q[e / 2]);
+                        v[t][e] = y.x, v[t][e + 1] = y.y;
                     }
-                } else if (on) {
-#pragma unroll
-                    for (int e = 0; e < 4; e += 2)
-                        if (4 * c + e < rot) {
-                            const float2 y = rope_turn(v[t][e], v[t][e + 1], __ldg(tab + 2 * c + e / 2));
-                            v[t][e] = y.x, v[t][e + 1] = y.y;
-                        }
                 }
-            } else if (on) {  // halves that do not fall on whole lanes: the partner from memory
-                const T* xr = x + (size_t)(t - first) * a.x[side].row;
+            }
+        }
+    } else if (TURN == kTurnAny && rot) {
+        for (int t = 0; t < kPage; t++) {
+            if (!in(t)) continue;
+            const T* xr = x + (size_t)(t - first) * ld;
+            const float2* tab = a.rope.table + (size_t)(pos0 + t) * half;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int d = 4 * c + e;
-                    if (d < half) v[t][e] = rope_turn(v[t][e], to_f32(xr[d + half]), tab[d]).x;
-                    else if (d < rot) v[t][e] = rope_turn(to_f32(xr[d - half]), v[t][e], tab[d - half]).y;
-                }
+            for (int e = 0; e < 4; e++) {
+                const int d = 4 * c + e;
+                if (d >= rot) continue;
+                const bool lo = a.rope.half ? d < half : !(d & 1);
+                const int p = a.rope.half ? (lo ? d + half : d - half) : d ^ 1;
+                const float2 cs = tab[a.rope.half ? (lo ? d : p) : d / 2];
+                const float mine = to_f32(xr[d]), other = to_f32(xr[p]);
+                const float y = lo ? rope_turn(mine, other, cs).x : rope_turn(other, mine, cs).y;
+#pragma unroll
+                for (int k = 0; k < kPage; k++)
+                    if (k == t) v[k][e] = y;
             }
         }
     }
@@ -493,7 +523,8 @@ static Kv8Cache cache_view(const pox_kv8_cache* c) {
     return Kv8Cache{c->pages, c->scales, c->num_blocks, (int)c->kv_heads};
 }
 static Kv8Batch batch_view(const pox_kv8_batch* b) {
-    return Kv8Batch{b->row_starts, b->ctx_lens, b->block_tables, b->seqs, b->rows, b->max_rows, b->max_ctx,
+    // as many rows as sequences and at most one each: one each, and no search on the device
+    return Kv8Batch{b->max_rows == 1 && b->rows == b->seqs ? nullptr : b->row_starts, b->ctx_lens, b->block_tables, b->seqs, b->rows, b->max_rows, b->max_ctx,
                     b->max_blocks_per_seq};
 }
 
@@ -571,7 +602,7 @@ static cudaError_t launch_qk(pox_cuda_ctx* ctx, const pox_qk_norm_rope* a, cudaS
 }
 
 static uint32_t page_items(const pox_kv8_batch* b) {
-    return b->row_starts ? (uint32_t)((b->rows + 30ull * b->seqs) / 16) : b->seqs;
+    return batch_view(b).row_starts ? (uint32_t)((b->rows + 30ull * b->seqs) / 16) : b->seqs;
 }
 // four elements of any (row, head) at once
 static int vec4(const pox_rows* r) {
@@ -585,7 +616,13 @@ static cudaError_t launch_append(pox_cuda_ctx* ctx, const pox_kv8_cache* c, cons
                     ctx->err_dev};
     const uint32_t items = page_items(b);
     const unsigned long long lanes = (unsigned long long)items * c->kv_heads * 2 * (HD / 4);
-    kv8_append_kernel<HD, T><<<(unsigned)((lanes + 127) / 128), 128, 0, st>>>(a, items, vec4(k) && vec4(v));
+    const unsigned grid = (unsigned)((lanes + 127) / 128);
+    const RopeView& r = a.rope;
+    const bool vec = vec4(k) && vec4(v) && ((uintptr_t)r.table & 15) == 0;
+    if (vec && !r.rot) kv8_append_kernel<HD, T, kTurnNone><<<grid, 128, 0, st>>>(a, items);
+    else if (vec && r.half && r.rot % 8 == 0) kv8_append_kernel<HD, T, kTurnHalf><<<grid, 128, 0, st>>>(a, items);
+    else if (vec && !r.half && r.rot % 4 == 0) kv8_append_kernel<HD, T, kTurnPairs><<<grid, 128, 0, st>>>(a, items);
+    else kv8_append_kernel<HD, T, kTurnAny><<<grid, 128, 0, st>>>(a, items);
     return cudaGetLastError();
 }
 

@@ -28,6 +28,23 @@ __device__ __forceinline__ float row_factor(float m, float& inverse) {
     return __uint_as_float((uint32_t)(127 + 13 - e) << 23);
 }
 
+// Four elements of a row as they lie.
+template <typename T>
+struct __align__(4 * sizeof(T)) Raw4 {
+    T v[4];
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T* x) {
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = x[i];
+        } else if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(x);
+        } else {
+            *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(x);
+        }
+    }
+};
+
 template <typename T>
 __device__ __forceinline__ void load4(const T* x, int vec, float (&v)[4]) {
     if (vec) {
