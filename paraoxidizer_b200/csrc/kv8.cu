@@ -67,102 +67,136 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(QkArgs<T> a) {
 // Bound by HBM (each element once in, once out), by the launch for a few rows. 16 bytes a load: of the L = hd / (2 V)
 // lanes of a head (V elements in 16 bytes), lane c holds the V dims from c V and the V dims from rot / 2 + c V, so that both
 // kinds of pairs lie within a lane, and what is not rotated in order behind. A warp takes 32 / L heads of a row at once and
-// `steps` such groups of it, two in flight, and keeps the row's (cos, sin) meanwhile.
-template <typename T, int L>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs<T> a, int steps, int groups) {
-    constexpr int V = 16 / sizeof(T), HW = 32 / L;
+// `steps` such groups of it and keeps the row's cosines and sines and the norm's weights meanwhile. kQkAhead groups are on
+// their way to shared memory, each lane's pieces to a place of its own (held in registers, two of them left too few
+// bytes in flight for HBM). All arithmetic goes two elements to an instruction: at one each, the issue slots
+// were as busy as the memory.
+constexpr int kQkAhead = 4;
+template <typename T, int L, bool HALF>
+__global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(QkArgs<T> a, int steps, int groups) {
+    constexpr int V = 16 / sizeof(T), HW = 32 / L, P = V / 2;
     const int lane = threadIdx.x & 31, c = lane % L, nh = a.heads[0] + a.heads[1], rot = a.rope.rot;
     const unsigned long long item = (unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const uint32_t r = (uint32_t)(item / groups);
     if (r >= a.rows) return;
     const int h0 = (int)(item % groups) * steps * HW + lane / L, turn = c < rot / (2 * V);
     const int d0 = turn ? c * V : 2 * c * V, d1 = turn ? rot / 2 + c * V : d0 + V;
+    const T* src[2] = {a.in[0].at(r, 0), a.in[1].at(r, 0)};
+    __shared__ uint4 ahead[kQkAhead][2][256];
+    auto fetch = [&](int k) {
+        const int h = h0 + k * HW, side = h >= a.heads[0];
+        if (k < steps && h < nh) {
+            const T* p = (side ? src[1] : src[0]) + (size_t)(h - (side ? a.heads[0] : 0)) * a.in[side].head;
+            cp16(smem_u32(&ahead[k % kQkAhead][0][threadIdx.x]), p + d0);
+            cp16(smem_u32(&ahead[k % kQkAhead][1][threadIdx.x]), p + d1);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int k = 0; k < kQkAhead; k++) fetch(k);
     const uint32_t p = rot ? a.pos[r] : 0;
     if (rot && p >= a.rope.positions) {
         if (lane == 0) atomicOr(a.err, kErrRopePos);
         return;
     }
-    // the pair index of element i of the lower piece (and, interleaved, of the upper one)
-    __align__(16) float2 cs[V];
+    // HALF: cosines and sines of the V pairs, two to a register pair. Else (cos, sin) and (-sin, cos) of each of them: the
+    // pairs of the lower piece, then of the upper one.
+    uint64_t cs[V], sn[HALF ? 1 : V];
     if (turn) {
-        const float4* t = reinterpret_cast<const float4*>(a.rope.table + (size_t)p * (rot / 2));
-        float4* q = reinterpret_cast<float4*>(cs);
+        const float2* t = a.rope.table + (size_t)p * (rot / 2);
+        if constexpr (HALF) {
 #pragma unroll
-        for (int i = 0; i < V / 2; i++)
-            q[i] = __ldg(t + (a.rope.half ? c * V / 2 + i : i < V / 4 ? c * V / 4 + i : (rot / 2 + c * V) / 4 + i - V / 4));
-    }
-    const T* src[2];
-    T* dst[2];
-    uint4 x[2][2];
-    auto fetch = [&](int k, int i) {
-        const int h = h0 + k * HW, side = h >= a.heads[0];
-        if (k < steps && h < nh) {
-            src[i] = a.in[side].at(r, h - (side ? a.heads[0] : 0));
-            dst[i] = a.out[side].at(r, h - (side ? a.heads[0] : 0));
-            x[i][0] = *reinterpret_cast<const uint4*>(src[i] + d0);
-            x[i][1] = *reinterpret_cast<const uint4*>(src[i] + d1);
-        }
-    };
-    auto finish = [&](int k, int i) {
-        const int h = h0 + k * HW, side = h >= a.heads[0];
-        const bool live = k < steps && h < nh;
-        float v[2][V];
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int e = 0; e < V; e++) v[u][e] = live ? to_f32(reinterpret_cast<const T*>(&x[i][u])[e]) : 0.f;
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < V; e++) ss = fmaf(v[0][e], v[0][e], fmaf(v[1][e], v[1][e], ss));
-#pragma unroll
-        for (int o = L / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (!live) return;
-        const __half* w = a.w[side];
-        if (w) {
-            const float inv = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
-            __align__(16) __half g[2][V];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const __half* q = w + (u ? d1 : d0);
-                if constexpr (V == 8) *reinterpret_cast<uint4*>(g[u]) = __ldg(reinterpret_cast<const uint4*>(q));
-                else *reinterpret_cast<uint2*>(g[u]) = __ldg(reinterpret_cast<const uint2*>(q));
+            for (int i = 0; i < P; i++) {
+                const float4 q = __ldg(reinterpret_cast<const float4*>(t + c * V) + i);
+                cs[i] = pair2(q.x, q.z);
+                cs[P + i] = pair2(q.y, q.w);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float2 q = __ldg(t + (i < P ? c * P + i : (rot / 2 + c * V) / 2 + i - P));
+                cs[i] = pair2(q.x, q.y);
+                sn[i] = pair2(-q.y, q.x);
+            }
+        }
+    }
+    uint64_t w[2][P];
+    int wside = -1;
+    auto finish = [&](int k) {
+        const int h = h0 + k * HW, side = h >= a.heads[0];
+        const bool live = h < nh;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kQkAhead - 1) : "memory");
+        uint64_t v[2][P], ss = 0;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const uint4 x = live ? ahead[k % kQkAhead][u][threadIdx.x] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < P; e++) {
+                v[u][e] = pair2(elem16<T>(x, 2 * e), elem16<T>(x, 2 * e + 1));
+                ss = fma2(v[u][e], v[u][e], ss);
+            }
+        }
+        float sum = both(ss).x + both(ss).y;
+#pragma unroll
+        for (int o = L / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (!live) return;
+        if (a.w[side]) {
+            if (side != wside) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const uint32_t* q = reinterpret_cast<const uint32_t*>(a.w[side] + (u ? d1 : d0));
+#pragma unroll
+                    for (int e = 0; e < P; e++) {
+                        const uint32_t g = __ldg(q + e);
+                        const float2 f = unpack_f16(g);
+                        w[u][e] = pair2(f.x, f.y);
+                    }
+                }
+                wside = side;
+            }
+            // 1 / sqrt by the approximation and one step of Newton's method
+            const float y = sum / (float)a.hd + a.eps, z = rsqrtf(y);
+            const float inv = y > 0x1p-120f && y < INFINITY ? fmaf(0.5f * z, fmaf(-y * z, z, 1.0f), z) : 1.0f / sqrtf(y);
+            const uint64_t f = pair2(inv, inv);
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int e = 0; e < V; e++) v[u][e] = v[u][e] * inv * __half2float(g[u][e]);
+                for (int e = 0; e < P; e++) v[u][e] = mul2(mul2(v[u][e], f), w[u][e]);
         }
         if (turn) {
-            if (a.rope.half) {
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float2 y = rope_turn(v[0][e], v[1][e], cs[e]);
-                    v[0][e] = y.x, v[1][e] = y.y;
-                }
-            } else {
+            for (int e = 0; e < P; e++) {
+                if constexpr (HALF) {
+                    const uint64_t lo = v[0][e], hi = v[1][e], z = mul2(hi, cs[P + e]);
+                    v[0][e] = fma2(lo, cs[e], z ^ 0x8000000080000000ull);
+                    v[1][e] = fma2(lo, cs[P + e], mul2(hi, cs[e]));
+                } else {
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        const float2 y = rope_turn(v[u][e], v[u][e + 1], cs[u * (V / 2) + e / 2]);
-                        v[u][e] = y.x, v[u][e + 1] = y.y;
+                    for (int u = 0; u < 2; u++) {  // (a, b) -> a (cos, sin) + b (-sin, cos)
+                        const float2 y = both(v[u][e]);
+                        v[u][e] = fma2(pair2(y.x, y.x), cs[u * P + e], mul2(pair2(y.y, y.y), sn[u * P + e]));
                     }
+                }
             }
         }
+        T* y = a.out[side].at(r, h - (side ? a.heads[0] : 0));
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            __align__(16) T t[V];
+            uint32_t t[4];
 #pragma unroll
-            for (int e = 0; e < V; e++) t[e] = from_f32<T>(v[u][e]);
-            *reinterpret_cast<uint4*>(dst[i] + (u ? d1 : d0)) = *reinterpret_cast<const uint4*>(t);
+            for (int e = 0; e < P; e++) {
+                const float2 q = both(v[u][e]);
+                if constexpr (sizeof(T) == 4) t[2 * e] = __float_as_uint(q.x), t[2 * e + 1] = __float_as_uint(q.y);
+                else t[e] = pack2<T>(q.x, q.y);
+            }
+            *reinterpret_cast<uint4*>(y + (u ? d1 : d0)) = make_uint4(t[0], t[1], t[2], t[3]);
         }
     };
-    for (int k = 0; k < steps; k += 2) {
-        fetch(k, 0);
-        fetch(k + 1, 1);
-        finish(k, 0);
-        finish(k + 1, 1);
+    for (int k = 0; k < steps; k++) {
+        finish(k);
+        fetch(k + kQkAhead);  // into the place just read
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---- append ----------------------------------------------------------------------------------------
@@ -181,46 +215,63 @@ __device__ __forceinline__ uint32_t page_base(const Kv8Batch& b, uint32_t s) {
     return !b.row_starts ? s : (uint32_t)(((unsigned long long)b.row_starts[s] + 30ull * s) / 16);
 }
 
-// What a unit of the append and read kernels works on: one page of one kv head, k or v, by a group of HD / 4
-// lanes, lane c of it on dims 4 c .. 4 c + 3 of all 16 tokens.
+// What a unit of the append and read kernels works on: one page of one kv head, k or v.
 struct PageUnit {
     SeqSpan sp;
     int page, first, last;  // its slots first .. last - 1 are rows of the batch
     size_t row;             // the row of slot `first`
+    int blk;                // its block-table entry as found
     int8_t* bytes;          // the page of the kv head
     float* scale;
 };
-template <int HD>
-__device__ __forceinline__ bool page_unit(const Kv8Cache& c, const Kv8Batch& b, uint32_t item, int h, int side, PageUnit& o,
-                                          int* err) {
-    const uint32_t s = b.row_starts ? find_seq<HD / 4>(b, item, 30, 16) : item;
+// The unit of page item `item`, its entry loaded but not looked at; false (reported) if the batch is at fault.
+// W lanes work on the unit together. A sequence without a page of that number has first >= last.
+template <int W>
+__device__ __forceinline__ bool page_unit(const Kv8Batch& b, uint32_t item, PageUnit& o, int* err) {
+    const uint32_t s = b.row_starts ? find_seq<W>(b, item, 30, 16) : item;
+    o.first = kPage, o.last = 0, o.page = 0, o.row = 0, o.blk = 0, o.bytes = nullptr;
     if (!seq_span(b, s, o.sp, err)) return false;
     const int begin = o.sp.ctx - o.sp.n, p0 = max(begin, 0);
     const int j = (int)(item - page_base(b, s));
     if (j < 0) {  // row_starts does not begin at 0
-        if ((threadIdx.x & (HD / 4 - 1)) == 0) atomicOr(err, kErrBatch);
+        if (threadIdx.x % W == 0) atomicOr(err, kErrBatch);
         return false;
     }
     o.page = p0 / kPage + j;
+    if (o.sp.ctx <= p0 || o.page * kPage >= o.sp.ctx) return true;
     o.first = max(p0 - o.page * kPage, 0), o.last = min(o.sp.ctx - o.page * kPage, kPage);
     o.row = (size_t)o.sp.r0 + (o.page * kPage + o.first - begin);
-    o.bytes = nullptr;
-    if (o.sp.ctx <= p0 || o.page * kPage >= o.sp.ctx) return true;
-    const int blk = b.btab[(size_t)s * b.mbps + o.page];
-    if (blk < 0 || (uint32_t)blk >= c.num_blocks) {
-        if ((threadIdx.x & (HD / 4 - 1)) == 0) atomicOr(err, kErrAttnPage);
+    o.blk = b.btab[(size_t)s * b.mbps + o.page];
+    return true;
+}
+// Where the unit's page lies; false (reported) if the entry is out of range.
+template <int HD>
+__device__ __forceinline__ bool page_resolve(const Kv8Cache& c, int h, int side, PageUnit& o, int* err) {
+    if (o.first >= o.last) return false;
+    if (o.blk < 0 || (uint32_t)o.blk >= c.num_blocks) {
+        atomicOr(err, kErrAttnPage);
         return false;
     }
-    o.bytes = c.pages + ((size_t)blk * c.kvh + h) * (2 * kPage * HD);
-    o.scale = c.scales + ((size_t)blk * c.kvh + h) * 2 + side;
+    const size_t p = (size_t)o.blk * c.kvh + h;
+    o.bytes = c.pages + p * (2 * kPage * HD);
+    o.scale = c.scales + p * 2 + side;
     return true;
 }
 
-// rint(x / s) as a byte: the quotient by Markstein's method (a correctly rounded reciprocal, one residual), the rounding by
-// adding 1.5 * 2^23, whose sum's low byte is the two's complement of the whole number.
-__device__ __forceinline__ uint32_t quantise(float x, float s, float rs) {
-    const float y = __fmul_rn(x, rs);
-    return __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-y, s, x), rs, y), 12582912.0f));
+// The larger of m and |x|, NaN if either is one.
+__device__ __forceinline__ float max_abs(float m, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
+}
+
+// rint(x / s) as a byte, two at once (low 8 bits of q0 and q1): the quotient by Markstein's method (y = x r with r the
+// rounded reciprocal, then y + (x - y s) r), the rounding by adding 1.5 * 2^23, whose sum's low byte is the two's
+// complement of the whole number. s2 = (-s, -s), r2 = (r, r).
+__device__ __forceinline__ void quantise2(float x0, float x1, uint64_t s2, uint64_t r2, uint32_t& q0, uint32_t& q1) {
+    const uint64_t x = pair2(x0, x1), y = mul2(x, r2);
+    const uint64_t z = add2(fma2(fma2(y, s2, x), r2, y), pair2(12582912.0f, 12582912.0f));
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(q0), "=r"(q1) : "l"(z));
 }
 __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return prmt(prmt(a, b, 0x0040), prmt(c, d, 0x0040), 0x5410);
@@ -230,50 +281,51 @@ __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t 
 // four elements at once and turn pairs within a lane (interleaved) or between lanes (halves of whole lanes).
 enum { kTurnAny = 0, kTurnNone = 1, kTurnHalf = 2, kTurnPairs = 3 };
 
-// Bound by HBM: rows in once, bytes out once. The page's new rows set the scale (a maximum over the group's lanes), its
-// older slots follow if the scale grew. All rows of a page are in flight at once; a lane's four dims make a word of each K
-// row and 64 contiguous bytes of V.
+// Bound by HBM: rows in once, bytes out once. A unit (page, kv head, side) is taken by two groups of HD / 4 lanes, lane c
+// of group `hi` on dims 4 c .. 4 c + 3 of tokens 8 hi .. 8 hi + 7, whose rows are all in flight at once (with all 16
+// tokens on a lane, 168 registers left 12 warps to an SM, and the loads' latency showed: 46 us for a 16381-token f32 prompt).
+// The page's new rows set the scale, its older slots follow if the scale grew. A lane's four dims make a word of
+// each K row and 8 bytes of each of four V rows.
 template <int HD, typename T, int TURN>
-__global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32_t items) {
-    constexpr int L = HD / 4, UW = 32 / L;
-    const int lane = threadIdx.x & 31, c = lane % L;
-    const unsigned long long u = ((unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * UW + lane / L;
+__global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uint32_t items) {
+    constexpr int L = HD / 4, UC = 128 / (2 * L), NT = kPage / 2;
+    __shared__ float red[4];
+    const int lane = threadIdx.x & 31, c = threadIdx.x % L, hi = threadIdx.x / L & 1, t0 = NT * hi;
+    const unsigned long long u = (unsigned long long)blockIdx.x * UC + threadIdx.x / (2 * L);
     const uint32_t item = min((uint32_t)(u / (2 * a.c.kvh)), items - 1);
     const int h = (int)(u % a.c.kvh), side = (int)(u / a.c.kvh % 2);
     PageUnit o;
-    bool live = u < (unsigned long long)items * 2 * a.c.kvh;
-    live = page_unit<HD>(a.c, a.b, item, h, side, o, a.err) && live && o.bytes;
-    const int rot = TURN == kTurnNone || side ? 0 : a.rope.rot, half = rot / 2, pos0 = o.page * kPage;
-    if (live && rot && (uint32_t)(pos0 + o.last - 1) >= a.rope.positions) {
+    bool live = page_unit<L>(a.b, item, o, a.err) && u < (unsigned long long)items * 2 * a.c.kvh && o.first < o.last;
+    const int rot = TURN == kTurnNone || side ? 0 : a.rope.rot, half = rot / 2, pos0 = o.page * kPage + t0;
+    if (live && rot && (uint32_t)(o.page * kPage + o.last - 1) >= a.rope.positions) {
         if (c == 0) atomicOr(a.err, kErrRopePos);
         live = false;
     }
-    const int first = live ? o.first : 0, last = live ? o.last : 0;
+    const int first = live ? o.first - t0 : 0, last = live ? o.last - t0 : 0;  // in this lane's tokens
     auto in = [&](int t) { return t >= first && t < last; };
-    const T* x = a.x[side].at(live ? o.row : 0, h);
     const size_t ld = a.x[side].row;
-    float v[kPage][4];
-    {
-        Raw4<T> raw[kPage];
+    const T* x = a.x[side].at(live ? o.row : 0, h) - (ptrdiff_t)first * (ptrdiff_t)ld;  // of token t0, if it is a row
+    Raw4<T> raw[NT];
 #pragma unroll
-        for (int t = 0; t < kPage; t++)
-            if (in(t)) raw[t].template load<TURN != kTurnAny>(x + (size_t)(t - first) * ld + 4 * c);
-#pragma unroll
-        for (int t = 0; t < kPage; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[t][e] = in(t) ? to_f32(raw[t].v[e]) : 0.f;
-    }
-    const float old = live && first ? *o.scale : 0.f;
-    uint4 ov[4];  // older bytes of V (a lane's dims), where the page is not written whole
-    const bool whole = first == 0 && last == kPage;
+    for (int t = 0; t < NT; t++)
+        if (in(t)) raw[t].template load<TURN != kTurnAny>(x + t * (ptrdiff_t)ld + 4 * c);
+    live = live && page_resolve<HD>(a.c, h, side, o, a.err);
+    const bool whole = o.first == 0 && o.last == kPage;
+    const float old = live && o.first ? *o.scale : 0.f;
+    uint2 ov[4];  // older bytes of V (this lane's dims and tokens), where the page is not written whole
     if (live && side && !whole)
 #pragma unroll
-        for (int e = 0; e < 4; e++) ov[e] = *reinterpret_cast<const uint4*>(o.bytes + kv8_v_off<HD>(0, 4 * c + e));
+        for (int e = 0; e < 4; e++) ov[e] = *reinterpret_cast<const uint2*>(o.bytes + kv8_v_off<HD>(t0, 4 * c + e));
+    float v[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[t][e] = in(t) ? to_f32(raw[t].v[e]) : 0.f;
     if constexpr (TURN == kTurnHalf || TURN == kTurnPairs) {
         const bool mine = 4 * c < rot, low = 4 * c < half;
         const int from = !mine ? lane : low ? lane + rot / 8 : lane - rot / 8;
 #pragma unroll
-        for (int tc = 0; tc < kPage; tc += 4) {  // (cos, sin) of four rows in flight
+        for (int tc = 0; tc < NT; tc += 4) {  // (cos, sin) of four rows in flight
             if (!__any_sync(0xffffffffu, rot && last > tc && first < tc + 4)) continue;
             float4 cs[4][2];
 #pragma unroll
@@ -296,8 +348,8 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32
                     for (int e = 0; e < 4; e++) w[e] = __shfl_sync(0xffffffffu, v[t][e], from);
                     if (mine && in(t))
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            v[t][e] = low ? rope_turn(v[t][e], w[e], q[e]).x : rope_turn(w[e], v[t][e], q[e]).y;
+                        for (int e = 0; e < 4; e++)  // rope_turn's half that this lane keeps
+                            v[t][e] = __fadd_rn(__fmul_rn(v[t][e], q[e].x), __fmul_rn(w[e], low ? -q[e].y : q[e].y));
                 } else if (mine && in(t)) {
 #pragma unroll
                     for (int e = 0; e < 4; e += 2) {
@@ -308,9 +360,10 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32
             }
         }
     } else if (TURN == kTurnAny && rot) {
-        for (int t = 0; t < kPage; t++) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
             if (!in(t)) continue;
-            const T* xr = x + (size_t)(t - first) * ld;
+            const T* xr = x + t * (ptrdiff_t)ld;
             const float2* tab = a.rope.table + (size_t)(pos0 + t) * half;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -319,44 +372,54 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32
                 const bool lo = a.rope.half ? d < half : !(d & 1);
                 const int p = a.rope.half ? (lo ? d + half : d - half) : d ^ 1;
                 const float2 cs = tab[a.rope.half ? (lo ? d : p) : d / 2];
-                const float mine = to_f32(xr[d]), other = to_f32(xr[p]);
-                const float y = lo ? rope_turn(mine, other, cs).x : rope_turn(other, mine, cs).y;
-#pragma unroll
-                for (int k = 0; k < kPage; k++)
-                    if (k == t) v[k][e] = y;
+                const float own = to_f32(xr[d]), other = to_f32(xr[p]);
+                v[t][e] = lo ? rope_turn(own, other, cs).x : rope_turn(other, own, cs).y;
             }
         }
     }
-    // the largest magnitude by its bits: what is not finite shows as the largest of all
-    uint32_t m = 0;
+    // the unit's largest magnitude: over the lanes of both groups
+    auto joined = [&](float m) {
 #pragma unroll
-    for (int t = 0; t < kPage; t++)
+        for (int k = (L == 32 ? 16 : L); k; k >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, k));
+        if constexpr (L == 32) {
+            if (lane == 0) red[threadIdx.x >> 5] = m;
+            __syncthreads();
+            m = max_abs(m, red[threadIdx.x >> 5 ^ 1]);
+        }
+        return m;
+    };
+    float m = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(v[t][e]) & 0x7fffffffu);
+    for (int t = 0; t < NT; t++)
 #pragma unroll
-    for (int k = L / 2; k; k >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
-    if (__any_sync(0xffffffffu, m >= 0x7f800000u)) {  // rare: infinities saturate, NaN is 0, neither sets the scale
-        m = 0;
+        for (int e = 0; e < 4; e++) m = max_abs(m, v[t][e]);
+    m = joined(m);
+    // rare: infinities saturate, NaN is 0, neither sets the scale; and scales whose reciprocal would leave the range
+    float up = 1.f;
+    if (__syncthreads_or(!(m < 0x1p120f) || (m > 0.f && m < 0x1p-90f) || (old > 0.f && old < 0x1p-100f))) {
+        m = 0.f;
 #pragma unroll
-        for (int t = 0; t < kPage; t++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (fabsf(v[t][e]) < INFINITY) m = max(m, __float_as_uint(v[t][e]) & 0x7fffffffu);
+                if (fabsf(v[t][e]) < INFINITY) m = fmaxf(m, fabsf(v[t][e]));
+        m = joined(m);
+        const float now = fmaxf(old, __fdiv_rn(m, 127.f));
+        up = now < 0x1p-64f ? 0x1p64f : now > 0x1p64f ? 0x1p-64f : 1.f;
 #pragma unroll
-        for (int k = L / 2; k; k >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
-        const float now = fmaxf(old, __fdiv_rn(__uint_as_float(m), 127.f));
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int t = 0; t < kPage; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                v[t][e] = v[t][e] == v[t][e] ? fminf(fmaxf(v[t][e], -127.f * now), 127.f * now) : 0.f;
+            for (int e = 0; e < 4; e++) {
+                const float y = v[t][e];
+                v[t][e] = y != y ? 0.f : fabsf(y) < INFINITY ? y * up : copysignf(127.f * (now * up), y);
+            }
     }
     if (!live) return;
-    const float now = fmaxf(old, __fdiv_rn(__uint_as_float(m), 127.f));
-    const bool grew = first && now > old;
+    const float now = fmaxf(old, __fdiv_rn(m, 127.f));
+    const bool grew = o.first && now > old;
     const float ratio = grew ? __fdiv_rn(old, now) : 1.f;
-    // a scale so small that its reciprocal overflows or is not exact enough: both sides times 2^64
-    const float up = now < 0x1p-100f ? 0x1p64f : 1.f, s = now > 0.f ? now * up : 1.f, rs = __frcp_rn(s);
+    const float s = now > 0.f ? now * up : 1.f, rs = __frcp_rn(s);
+    const uint64_t s2 = pair2(-s, -s), r2 = pair2(rs, rs);
     auto older = [&](uint32_t w, int n) {  // the first n bytes of a word to the new scale
         uint32_t q[4];
 #pragma unroll
@@ -367,45 +430,49 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(AppendArgs<T> a, uint32
     };
     if (side == 0) {
         if (grew)
-            for (int t = 0; t < first; t++) {
-                uint32_t* w = reinterpret_cast<uint32_t*>(o.bytes + kv8_k_off<HD>(t, 4 * c));
+            for (int t = 0; t < min(first, NT); t++) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(o.bytes + kv8_k_off<HD>(t0 + t, 4 * c));
                 *w = older(*w, 4);
             }
 #pragma unroll
-        for (int t = 0; t < kPage; t++)
-            if (t >= first && t < last) {
+        for (int t = 0; t < NT; t++)
+            if (in(t)) {
                 uint32_t q[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) q[e] = quantise(v[t][e] * up, s, rs);
-                *reinterpret_cast<uint32_t*>(o.bytes + kv8_k_off<HD>(t, 4 * c)) = pack_bytes(q[0], q[1], q[2], q[3]);
+                quantise2(v[t][0], v[t][1], s2, r2, q[0], q[1]);
+                quantise2(v[t][2], v[t][3], s2, r2, q[2], q[3]);
+                *reinterpret_cast<uint32_t*>(o.bytes + kv8_k_off<HD>(t0 + t, 4 * c)) = pack_bytes(q[0], q[1], q[2], q[3]);
             }
-    } else {
+    } else if (whole || grew || (first < NT && last > 0)) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            uint32_t w[4];
+        for (int e = 0; e < 4; e += 2) {
+            uint32_t w[2][2];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint32_t b = whole ? 0u : k == 0 ? ov[e].x : k == 1 ? ov[e].y : k == 2 ? ov[e].z : ov[e].w;
-                uint32_t q[4];
+            for (int k = 0; k < 2; k++) {
+                uint32_t q[2][4];
 #pragma unroll
-                for (int t = 0; t < 4; t++) q[t] = quantise(v[4 * k + t][e] * up, s, rs);
-                w[k] = pack_bytes(q[0], q[1], q[2], q[3]);
-                if (!whole) {
-                    const uint32_t keep = grew ? older(b, first - 4 * k) : b;
-                    uint32_t mask = 0;  // bytes of slots first .. last - 1
+                for (int t = 0; t < 4; t++) quantise2(v[4 * k + t][e], v[4 * k + t][e + 1], s2, r2, q[0][t], q[1][t]);
 #pragma unroll
-                    for (int t = 0; t < 4; t++) mask |= 4 * k + t >= first && 4 * k + t < last ? 0xffu << 8 * t : 0u;
-                    w[k] = (w[k] & mask) | (keep & ~mask);
+                for (int i = 0; i < 2; i++) {
+                    w[i][k] = pack_bytes(q[i][0], q[i][1], q[i][2], q[i][3]);
+                    if (!whole) {
+                        const uint32_t b = k ? ov[e + i].y : ov[e + i].x, keep = grew ? older(b, first - 4 * k) : b;
+                        uint32_t mask = 0;  // bytes of slots first .. last - 1
+#pragma unroll
+                        for (int t = 0; t < 4; t++) mask |= in(4 * k + t) ? 0xffu << 8 * t : 0u;
+                        w[i][k] = (w[i][k] & mask) | (keep & ~mask);
+                    }
                 }
             }
-            *reinterpret_cast<uint4*>(o.bytes + kv8_v_off<HD>(0, 4 * c + e)) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                *reinterpret_cast<uint2*>(o.bytes + kv8_v_off<HD>(t0, 4 * c + e + i)) = make_uint2(w[i][0], w[i][1]);
         }
     }
-    if (c == 0) *o.scale = now;
+    if (c == 0 && hi == 0) *o.scale = now;
 }
 
 // ---- reading rows back -------------------------------------------------------------------------------
-// The append's units the other way round. The unit of a sequence's first page also clears its padding rows.
+// The append's units the other way round, one group of HD / 4 lanes to all tokens of a unit. The unit of a sequence's first page also clears its padding rows.
 template <int HD, typename T>
 __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8Cache cache, Kv8Batch b, RowsView<T> k, RowsView<T> v,
                                                        uint32_t items, int vec, int* err) {
@@ -415,14 +482,14 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8Cache cache, Kv8Batch 
     const uint32_t item = min((uint32_t)(u / (2 * cache.kvh)), items - 1);
     const int h = (int)(u % cache.kvh), side = (int)(u / cache.kvh % 2);
     PageUnit o;
-    const bool ok = page_unit<HD>(cache, b, item, h, side, o, err);
+    const bool ok = page_unit<L>(b, item, o, err);
     if (!ok || u >= (unsigned long long)items * 2 * cache.kvh) return;
     const RowsView<T>& out = side ? v : k;
     const int begin = o.sp.ctx - o.sp.n;
     if (begin < 0 && o.page == 0)
         for (int i = 0; i < min(-begin, o.sp.n); i++)
             store4(out.at((size_t)o.sp.r0 + i, h) + 4 * c, vec, make_float4(0.f, 0.f, 0.f, 0.f));
-    if (!o.bytes) return;
+    if (!page_resolve<HD>(cache, h, side, o, err)) return;
     const float s = *o.scale;
     uint32_t w[kPage];  // K: the four dims of each token; V: four words of each dim
     if (side == 0) {
@@ -588,16 +655,21 @@ static cudaError_t launch_qk(pox_cuda_ctx* ctx, const pox_qk_norm_rope* a, cudaS
     // as many groups of heads to a warp as leave every SM its 32 warps
     const int all = (nh * L + 31) / 32;
     const int steps = (int)std::min<long long>(std::max<long long>((long long)a->rows * all / (32LL * ctx->num_sms), 1),
-                                               std::min(all, 8));
+                                               std::min(all, 10));
     const int groups = (all + steps - 1) / steps;
     const unsigned grid = (unsigned)(((unsigned long long)a->rows * groups + 7) / 8);
-    switch (L) {
-        case 2: qk_norm_rope_kernel<T, 2><<<grid, 256, 0, st>>>(k, steps, groups); break;
-        case 4: qk_norm_rope_kernel<T, 4><<<grid, 256, 0, st>>>(k, steps, groups); break;
-        case 8: qk_norm_rope_kernel<T, 8><<<grid, 256, 0, st>>>(k, steps, groups); break;
-        case 16: qk_norm_rope_kernel<T, 16><<<grid, 256, 0, st>>>(k, steps, groups); break;
-        default: qk_norm_rope_kernel<T, 32><<<grid, 256, 0, st>>>(k, steps, groups);
-    }
+    auto go = [&](auto half) {
+        constexpr bool H = decltype(half)::value;
+        switch (L) {
+            case 2: qk_norm_rope_kernel<T, 2, H><<<grid, 256, 0, st>>>(k, steps, groups); break;
+            case 4: qk_norm_rope_kernel<T, 4, H><<<grid, 256, 0, st>>>(k, steps, groups); break;
+            case 8: qk_norm_rope_kernel<T, 8, H><<<grid, 256, 0, st>>>(k, steps, groups); break;
+            case 16: qk_norm_rope_kernel<T, 16, H><<<grid, 256, 0, st>>>(k, steps, groups); break;
+            default: qk_norm_rope_kernel<T, 32, H><<<grid, 256, 0, st>>>(k, steps, groups);
+        }
+    };
+    if (k.rope.half) go(std::true_type());
+    else go(std::false_type());
     return cudaGetLastError();
 }
 
@@ -615,7 +687,7 @@ static cudaError_t launch_append(pox_cuda_ctx* ctx, const pox_kv8_cache* c, cons
     AppendArgs<T> a{cache_view(c), batch_view(b), {rows_view<const T>(*k), rows_view<const T>(*v)}, rope_view(rope),
                     ctx->err_dev};
     const uint32_t items = page_items(b);
-    const unsigned long long lanes = (unsigned long long)items * c->kv_heads * 2 * (HD / 4);
+    const unsigned long long lanes = (unsigned long long)items * c->kv_heads * 2 * (HD / 2);
     const unsigned grid = (unsigned)((lanes + 127) / 128);
     const RopeView& r = a.rope;
     const bool vec = vec4(k) && vec4(v) && ((uintptr_t)r.table & 15) == 0;

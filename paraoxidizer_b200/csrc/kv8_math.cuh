@@ -28,6 +28,56 @@ __device__ __forceinline__ float row_factor(float m, float& inverse) {
     return __uint_as_float((uint32_t)(127 + 13 - e) << 23);
 }
 
+// Two f32 operations in one instruction, each rounded as by itself.
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+
+// Two values rounded to the rows' type, as they lie.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+// Element i of 16 bytes of a row.
+template <typename T>
+__device__ __forceinline__ float elem16(const uint4& v, int i) {
+    const uint32_t w = sizeof(T) == 4 ? (i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w)
+                                      : (i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w);
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        return i & 1 ? f.y : f.x;
+    } else return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+}
+
 // Four elements of a row as they lie.
 template <typename T>
 struct __align__(4 * sizeof(T)) Raw4 {
@@ -70,6 +120,9 @@ __device__ __forceinline__ void store4(T* x, int vec, float4 v) {
     }
 }
 
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
