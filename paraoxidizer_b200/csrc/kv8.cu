@@ -600,7 +600,7 @@ constexpr int kPromptRows = 64;
 // The stream's split partials and tickets for a plan that splits.
 static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, uint32_t hd, Kv8StepPlan& p) {
     if (p.splits <= 1) return POX_OK;
-    const size_t need = p.items * p.splits * (p.pair ? 8 : 16) * (hd + 2) * sizeof(float);
+    const size_t need = p.items * p.splits * 8 * p.tiles * (hd + 2) * sizeof(float);
     try {
         std::lock_guard<std::mutex> lk(ctx->mu);
         Kv8Scratch& k = ctx->kv8[st];
@@ -823,7 +823,7 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     const long long most = (long long)b->max_rows * G;
     const bool prompt = c->head_dim != 32 && q->dtype != POX_F32 && most > kPromptRows;
     const bool step = !prompt || (b->seqs > 1 && b->rows != (unsigned long long)b->seqs * b->max_rows);
-    Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, G, q->dtype == POX_F32, ctx->num_sms,
+    Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, G, ctx->num_sms,
                                      prompt ? kPromptRows : 0x7fffffff);
     if (plan.items * (unsigned __int128)plan.splits > 0x7fffffffu)
         return set_error(POX_ERR_UNSUPPORTED, "%zu items of %d splits", plan.items, plan.splits);

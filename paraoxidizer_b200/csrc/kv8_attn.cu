@@ -10,21 +10,49 @@
 
 namespace pox {
 
-constexpr int kStepStages = 4;  // pages in flight per warp
+// Bytes of a page in the ring; pages in flight per warp (about 12 KB).
+template <int HD>
+struct StepRing {
+    static constexpr int kPageBytes = 32 * HD, kStages = HD == 128 ? 3 : HD == 64 ? 6 : 8;
+};
 
-// One CTA per (sequence, kv head, split of the context, tile of rows). Each warp streams whole pages (K and V of 16
-// tokens of the kv head, 32 HD contiguous bytes) through a ring of its own with one bulk copy a page, and runs both products on
-// mma.sync m16n8k16 with f32 accumulators: the rows are A, the int8 operands become exact f16 on the way from
-// shared memory. An MMA does not care in which order k runs, so the order is the one that the page's bytes
-// have: lane (g, t) takes 16 dims of a token for Q K^T and the four tokens 4 t .. 4 t + 3 of a dim for P V, and
-// the scores leave the first product where the second wants them.
-// PAIR: 8 rows, A rows g and g + 8 being the two f16 terms of row g (f32 rows need them; fewer rows
-// than 9 leave the place free). Otherwise 16 rows, p rounded to f16 (2^-11 of p, as the output's type).
-template <int HD, typename T, bool PAIR>
-__global__ void __launch_bounds__(32 * kStepWarps, 3) kv8_attn_step_kernel(Kv8Attn<T> a, Kv8StepPlan p) {
-    constexpr int RT = PAIR ? 8 : 16, KW = HD / 16, NJ = HD / 8, PB = 32 * HD, NR = PAIR ? 1 : 2;
+// Two f16 from the low (high) two bytes of a word of int8.
+//   EXACT: the whole numbers q themselves.
+//   else:  (q + 128) 2^-24, the byte with its sign bit flipped as a subnormal f16: three instructions a word instead of
+//          five; the products' sums are then off by 128 2^-24 times the sum of the other operand, which the caller takes off.
+template <bool EXACT>
+__device__ __forceinline__ void bytes_to_f16(uint32_t v, uint32_t& r0, uint32_t& r1) {
+    if constexpr (EXACT) {
+        i8x4_to_f16x4(v, r0, r1);
+    } else {
+        const uint32_t u = v ^ 0x80808080u;
+        r0 = prmt(u, 0u, 0x4140u);
+        r1 = prmt(u, 0u, 0x4342u);
+    }
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {  // an 8 x 8 matrix of f16 pairs across the warp
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// One CTA per (sequence, kv head, split of the context, tile of 8 NT rows). Each warp streams whole pages (K and V of
+// 16 tokens of the kv head, 32 HD contiguous bytes) through a ring of its own with one bulk copy a page, and runs both
+// products transposed on mma.sync m16n8k16 with f32 accumulators, so that a page is the 16 rows of A and 8 query rows fill N:
+//   S^T (tokens x rows) = K Q^T,   O^T (dims x rows) = V^T P^T.
+// The MMA does not care in which order k and the rows of A run, so they run as the page's bytes lie: lane (g, t) takes
+// 16 dims of the tokens 4 (g / 2) + g % 2 (+ 2) for the first product and the four tokens 4 t .. 4 t + 3 of a dim for the
+// second, and P^T is S^T's own fragment, transposed in registers.
+// f32 rows: q and p as two f16 terms each (22 bits), bytes converted exactly. 16-bit rows: q exact, bytes with the
+// offset of bytes_to_f16; p two terms for f16 outputs of up to 8 rows (so that only the output's own rounding
+// remains), one for bf16 and for more rows (2^-11 of p).
+template <int HD, typename T, int NT>
+__global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_step_kernel(Kv8Attn<T> a, Kv8StepPlan p) {
+    constexpr bool F32 = sizeof(T) == 4, PLO = F32 || (std::is_same<T, __half>::value && NT == 1);
+    constexpr int RT = 8 * NT, KW = HD / 16, NJ = HD / 16, PB = StepRing<HD>::kPageBytes, NST = StepRing<HD>::kStages;
+    constexpr float kOffset = 128.0f / 16777216.0f;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[kStepWarps][kStepStages];
+    __shared__ __align__(8) uint64_t bars[kStepWarps][NST];
     __shared__ float ml[kStepWarps][2][RT];
     __shared__ uint32_t last_cta;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -47,9 +75,9 @@ __global__ void __launch_bounds__(32 * kStepWarps, 3) kv8_attn_step_kernel(Kv8At
     // this warp's pages: first, first + W, ..; lane i holds the i-th one's place and scales
     const int first = sp * p.pages_per_split + warp, end = min(pages, (sp + 1) * p.pages_per_split);
     const int cnt = first < end ? (end - first + kStepWarps - 1) / kStepWarps : 0;
-    const uint32_t ring = smem_u32(smem) + warp * kStepStages * PB, bar = smem_u32(&bars[warp][0]);
+    const uint32_t ring = smem_u32(smem) + warp * NST * PB, bar = smem_u32(&bars[warp][0]);
     if (lane == 0) {
-        for (int i = 0; i < kStepStages; i++) mbar_init(bar + 8 * i, 1);
+        for (int i = 0; i < NST; i++) mbar_init(bar + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
@@ -62,28 +90,27 @@ __global__ void __launch_bounds__(32 * kStepWarps, 3) kv8_attn_step_kernel(Kv8At
         place = there ? (size_t)blk * a.c.kvh + h : 0;
     }
     const unsigned there_m = __ballot_sync(0xffffffffu, there);
-    auto fetch = [&](int i) {  // page i of this warp into its stage (a page out of range: page 0, unread)
+    auto fetch = [&](int i, int st) {  // page i of this warp into its stage (a page out of range: page 0, unread)
         const size_t pl = __shfl_sync(0xffffffffu, (unsigned long long)place, i);
         if (lane == 0) {
-            const int st = i % kStepStages;
             mbar_expect_tx(bar + 8 * st, PB);
             bulk_g2s(ring + st * PB, a.c.pages + pl * PB, PB, bar + 8 * st);
         }
     };
-    for (int i = 0; i < min(cnt, kStepStages); i++) fetch(i);
+    for (int i = 0; i < min(cnt, NST); i++) fetch(i, i);
     const float2 ab = lane < cnt ? *reinterpret_cast<const float2*>(a.c.scales + place * 2) : make_float2(0.f, 0.f);
     // log2 b; a scale of 0 stands for zeros whatever the bytes: 1e-30 of them is nothing next to any other page
     const float lb = log2f(fmaxf(ab.y, 1e-30f) + (ab.y - ab.y)), ib = 1.0f / fmaxf(ab.y, 1e-30f);
 
-    // A fragments of the rows, and what takes their products to scores
-    uint32_t qa[KW][4];
-    float qf[NR];
-    int rpos[NR];
+    // B fragments of the rows: lane (g, t) the dims of row g that t takes of a token. Then, for the rows 2 t and 2 t + 1 that
+    // this lane's scores belong to: what takes a product to a score, its offset, and the last position seen
+    uint32_t qb[NT][F32 ? 2 : 1][KW][2];
+    float qf[NT][2], qo[NT][2];
+    int rpos[NT][2];
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-        const int row = row0 + g + 8 * r;
+    for (int n = 0; n < NT; n++) {
+        const int row = row0 + 8 * n + g;
         const bool ok = row < rows;
-        rpos[r] = ok ? pos0 + row / a.G : 0;
         const T* q = a.q.at((size_t)sq.r0 + (ok ? row / a.G : 0), h * a.G + (ok ? row % a.G : 0));
         float v[KW][4], m = 0.f;
 #pragma unroll
@@ -94,146 +121,199 @@ __global__ void __launch_bounds__(32 * kStepWarps, 3) kv8_attn_step_kernel(Kv8At
 #pragma unroll
             for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(v[w][i]));
         }
-        float f = 1.f, inv = 1.f;
-        if constexpr (sizeof(T) == 4 || std::is_same<T, __nv_bfloat16>::value) {
+        float f = 1.f, inv = 1.f, sum = 0.f;
+        if constexpr (!std::is_same<T, __half>::value) {
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             f = row_factor(m, inv);
         }
-        qf[r] = inv * a.scale;
 #pragma unroll
         for (int w = 0; w < KW; w++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const float x = v[w][2 * i] * f, y = v[w][2 * i + 1] * f;
-                qa[w][2 * i + r] = pack_f16(x, y);
-                if constexpr (PAIR && sizeof(T) == 4) {
-                    const float2 hi = unpack_f16(qa[w][2 * i]);
-                    qa[w][2 * i + 1] = pack_f16(x - hi.x, y - hi.y);
-                } else if (PAIR) {
-                    qa[w][2 * i + 1] = 0u;
+                qb[n][0][w][i] = pack_f16(x, y);
+                if constexpr (F32) {
+                    const float2 hi = unpack_f16(qb[n][0][w][i]);
+                    qb[n][F32][w][i] = pack_f16(x - hi.x, y - hi.y);
+                } else {
+                    sum += x + y;  // (16-bit rows are f16 exactly)
                 }
             }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            qf[n][e] = __shfl_sync(0xffffffffu, inv, 8 * t + 4 * e) * a.scale * (F32 ? 1.0f : 16777216.0f);
+            qo[n][e] = F32 ? 0.f : -kOffset * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
+            const int r = row0 + 8 * n + 2 * t + e;
+            rpos[n][e] = r < rows ? pos0 + r / a.G : 0;
+        }
     }
 
-    float o[NJ][4], m[NR], l[NR];
+    float o[NT][NJ][4], m[NT][2], l[NT][2], ps[NT][2];  // ps: the sum of p as the product sees it
 #pragma unroll
-    for (int j = 0; j < NJ; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    for (int n = 0; n < NT; n++) {
 #pragma unroll
-    for (int r = 0; r < NR; r++) m[r] = -INFINITY, l[r] = 0.f;
+        for (int j = 0; j < NJ; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; e++) m[n][e] = -INFINITY, l[n][e] = 0.f, ps[n][e] = 0.f;
+    }
+    const int tok = 4 * (g >> 1) + (g & 1);
     bool bad = false;
+    int st = 0, ph = 0;
     for (int i = 0; i < cnt; i++) {
-        const int st = i % kStepStages, page = first + i * kStepWarps;
+        const int page = first + i * kStepWarps;
         const uint32_t base = ring + st * PB;
-        if (!bad) bad = __any_sync(0xffffffffu, !mbar_wait(bar + 8 * st, (i / kStepStages) & 1));
+        bad = __any_sync(0xffffffffu, !mbar_wait(bar + 8 * st, ph));
         const float pa = __shfl_sync(0xffffffffu, ab.x, i), pl = __shfl_sync(0xffffffffu, lb, i),
                     pi = __shfl_sync(0xffffffffu, ib, i);
-        float sc[2][4];
+        // S^T: tokens tok (rows g of A) and tok + 2 (rows g + 8); two chains of products
+        float sc[NT][2][4];
 #pragma unroll
-        for (int nb = 0; nb < 2; nb++) {
-            const int tok = 4 * (g >> 1) + 2 * nb + (g & 1);
-            sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-            uint32_t kw[KW];
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) sc[n][k][e] = k == 0 ? qo[n][e & 1] : 0.f;
+        uint32_t kw[2][KW];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const uint32_t at = base + (tok + 2 * u) * HD;
             if constexpr (HD == 32) {
-                const uint2 x = lds64(base + tok * HD + 8 * t);
-                kw[0] = x.x, kw[1] = x.y;
+                const uint2 x = lds64(at + 8 * t);
+                kw[u][0] = x.x, kw[u][1] = x.y;
             } else {
 #pragma unroll
                 for (int c = 0; c < HD / 64; c++) {
-                    const uint4 x = lds128(base + tok * HD + (HD == 128 ? (64 * c + 16 * t) ^ ((g & 1) << 6) : 16 * t));
-                    kw[4 * c] = x.x, kw[4 * c + 1] = x.y, kw[4 * c + 2] = x.z, kw[4 * c + 3] = x.w;
+                    const uint4 x = lds128(at + (HD == 128 ? (64 * c + 16 * t) ^ ((g & 1) << 6) : 16 * t));
+                    kw[u][4 * c] = x.x, kw[u][4 * c + 1] = x.y, kw[u][4 * c + 2] = x.z, kw[u][4 * c + 3] = x.w;
                 }
             }
+        }
 #pragma unroll
-            for (int w = 0; w < KW; w++) {
-                uint32_t b0, b1;
-                i8x4_to_f16x4(kw[w], b0, b1);
-                mma_16816(sc[nb], qa[w][0], qa[w][1], qa[w][2], qa[w][3], b0, b1);
+        for (int w = 0; w < KW; w++) {
+            uint32_t a0, a1, a2, a3;
+            bytes_to_f16<F32>(kw[0][w], a0, a2);
+            bytes_to_f16<F32>(kw[1][w], a1, a3);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                mma_16816(sc[n][w & 1], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1]);
+                if constexpr (F32) mma_16816(sc[n][w & 1], a0, a1, a2, a3, qb[n][F32][w][0], qb[n][F32][w][1]);
             }
         }
-        // u of tokens 4 t + 2 nb + e
-        const bool whole = page * kPage + kPage - 1 <= pmin && (there_m >> i & 1);
-        float u[NR][4], mx[NR];
+        // u of tokens tok, tok + 2 and rows 2 t, 2 t + 1
+        const bool seen = there_m >> i & 1, whole = page * kPage + kPage - 1 <= pmin && seen;
+        float u[NT][4];
         bool grow = false;
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            const float f = qf[r] * pa;
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float x = PAIR ? sc[e >> 1][e & 1] + sc[e >> 1][2 + (e & 1)] : sc[e >> 1][2 * r + (e & 1)];
-                u[r][e] = fmaf(x, f, pl);
-                if (!whole && (page * kPage + 4 * t + e > rpos[r] || !(there_m >> i & 1))) u[r][e] = -INFINITY;
+            for (int e = 0; e < 2; e++) {
+                const float f = qf[n][e] * pa;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    float x = fmaf(sc[n][0][2 * k + e] + sc[n][1][2 * k + e], f, pl);
+                    if (!whole && (page * kPage + tok + 2 * k > rpos[n][e] || !seen)) x = -INFINITY;
+                    u[n][2 * k + e] = x;
+                }
+                grow |= fmaxf(u[n][e], u[n][2 + e]) > m[n][e] + 8.0f;
             }
-            float y = fmaxf(fmaxf(u[r][0], u[r][1]), fmaxf(u[r][2], u[r][3]));
-            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
-            mx[r] = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-            grow |= mx[r] > m[r] + 8.0f;
-        }
         // the reference moves only when p would pass 2^8: after the first pages it hardly ever does
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int r = 0; r < NR; r++) {
-                const float to = mx[r] > m[r] + 8.0f ? mx[r] : m[r];
-                const float f = m[r] == -INFINITY ? (to == -INFINITY ? 1.f : 0.f) : ex2(m[r] - to);
-                m[r] = to;
-                l[r] *= f;
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    o[j][2 * r] *= f, o[j][2 * r + 1] *= f;
-                    if (PAIR) o[j][2] *= f, o[j][3] *= f;
+                for (int e = 0; e < 2; e++) {
+                    float to = fmaxf(u[n][e], u[n][2 + e]);
+#pragma unroll
+                    for (int k = 4; k < 32; k *= 2) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, k));
+                    to = to > m[n][e] + 8.0f ? to : m[n][e];
+                    const float f = m[n][e] == -INFINITY ? (to == -INFINITY ? 1.f : 0.f) : ex2(m[n][e] - to);
+                    m[n][e] = to;
+                    l[n][e] *= f, ps[n][e] *= f;
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) o[n][j][e] *= f, o[n][j][2 + e] *= f;
+                }
+        }
+        uint32_t pb[NT][PLO ? 2 : 1][2];  // B fragments of P^T: tokens 4 t, 4 t + 1 | 4 t + 2, 4 t + 3 of row g
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float x[4], y[2] = {0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = ex2(u[n][e] - (m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1]));
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const uint32_t hi = pack_f16(x[2 * k], x[2 * k + 1]);
+                const float2 r = unpack_f16(hi);
+                pb[n][0][k] = transpose8(hi);
+                if constexpr (PLO) {
+                    const uint32_t lo = pack_f16(x[2 * k] - r.x, x[2 * k + 1] - r.y);
+                    pb[n][PLO][k] = transpose8(lo);
+                    y[0] += x[2 * k], y[1] += x[2 * k + 1];
+                } else {
+                    y[0] += r.x, y[1] += r.y;
                 }
             }
-        }
-        uint32_t pp[4];  // A fragment of P: tokens 4 t, 4 t + 1 | 4 t + 2, 4 t + 3
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            const float ref = m[r] == -INFINITY ? 0.f : m[r];
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = ex2(u[r][e] - ref);
-            const float sum = (x[0] + x[1]) + (x[2] + x[3]);
-            if (sum != 0.f) l[r] = fmaf(sum, pi, l[r]);  // (an unseen page's scale may be anything)
-            pp[r] = pack_f16(x[0], x[1]);
-            pp[2 + r] = pack_f16(x[2], x[3]);
-            if (PAIR) {
-                const float2 h0 = unpack_f16(pp[0]), h1 = unpack_f16(pp[2]);
-                pp[1] = pack_f16(x[0] - h0.x, x[1] - h0.y);
-                pp[3] = pack_f16(x[2] - h1.x, x[3] - h1.y);
+            for (int e = 0; e < 2; e++) {
+                if (y[e] != 0.f) l[n][e] = fmaf(y[e], pi, l[n][e]);  // (an unseen page's scale may be anything)
+                if (!F32) ps[n][e] += y[e];
             }
         }
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            uint32_t w, b0, b1;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(base + kPage * HD + (8 * j + g) * kPage + 4 * t));
-            i8x4_to_f16x4(w, b0, b1);
-            mma_16816(o[j], pp[0], pp[1], pp[2], pp[3], b0, b1);
+            uint32_t w0, w1, a0, a1, a2, a3;
+            const uint32_t at = base + kPage * HD + (16 * j + g) * kPage + 4 * t;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0) : "r"(at));
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1) : "r"(at + 8 * kPage));
+            bytes_to_f16<F32>(w0, a0, a2);
+            bytes_to_f16<F32>(w1, a1, a3);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                mma_16816(o[n][j], a0, a1, a2, a3, pb[n][0][0], pb[n][0][1]);
+                if constexpr (PLO) mma_16816(o[n][j], a0, a1, a2, a3, pb[n][PLO][0], pb[n][PLO][1]);
+            }
         }
         __syncwarp();  // every lane has read the stage
-        if (i + kStepStages < cnt && !bad) fetch(i + kStepStages);
         if (bad) {  // a copy did not come in time: give the ones in flight as long again, and leave
-            for (int k = i; k < min(cnt, i + kStepStages); k++) mbar_wait(bar + 8 * (k % kStepStages), (k / kStepStages) & 1);
+            for (int k = i; k < min(cnt, i + NST); k++) {
+                mbar_wait(bar + 8 * st, ph);
+                if (++st == NST) st = 0, ph ^= 1;
+            }
             if (lane == 0) atomicOr(a.err, kErrWaitRing);
             break;
         }
+        if (i + NST < cnt) fetch(i + NST, st);
+        if (++st == NST) st = 0, ph ^= 1;
     }
 
     // the warps' parts: (m, l) and o in units of 2^m, through the ring's space
+    constexpr int OS = HD + 4;  // floats of a row there (rows 2 t of a warp's stores in distinct banks)
+    float off[NT][2];
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if (t == 0) ml[warp][0][g + 8 * r] = m[r], ml[warp][1][g + 8 * r] = l[r];
-    }
-    __syncthreads();
-    float* os = reinterpret_cast<float*>(smem);  // [warp][RT][HD]
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-    for (int j = 0; j < NJ; j++)
+        for (int e = 0; e < 2; e++) {
+            float y = l[n][e], z = ps[n][e];
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            const float2 x = PAIR ? make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3])
-                                  : make_float2(o[j][2 * r], o[j][2 * r + 1]);
-            *reinterpret_cast<float2*>(os + ((size_t)warp * RT + g + 8 * r) * HD + 8 * j + 2 * t) = x;
+            for (int k = 4; k < 32; k *= 2) {
+                y += __shfl_xor_sync(0xffffffffu, y, k);
+                if (!F32) z += __shfl_xor_sync(0xffffffffu, z, k);
+            }
+            if (g == 0) ml[warp][0][8 * n + 2 * t + e] = m[n][e], ml[warp][1][8 * n + 2 * t + e] = y;
+            off[n][e] = -128.0f * z;
         }
+    __syncthreads();
+    float* os = reinterpret_cast<float*>(smem);  // [warp][RT][OS]
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                os[((size_t)warp * RT + 8 * n + 2 * t + (e & 1)) * OS + 16 * j + 8 * (e >> 1) + g] =
+                    F32 ? o[n][j][e] : fmaf(o[n][j][e], 16777216.0f, off[n][e & 1]);
     __syncthreads();
     const size_t item = ((size_t)s * a.c.kvh + h) * p.row_tiles + rt;
     float* part = p.part + (item * p.splits + sp) * RT * (HD + 2);
@@ -248,7 +328,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, 3) kv8_attn_step_kernel(Kv8At
         for (int w = 0; w < kStepWarps; w++) {
             // NaN scores leave m at -inf with l NaN: the weight of such a part is 1, so that the row is NaN
             const float f = ml[w][0][r] == -INFINITY ? (ml[w][1][r] == 0.f ? 0.f : 1.f) : ex2(ml[w][0][r] - M);
-            const float4 y = *reinterpret_cast<const float4*>(os + ((size_t)w * RT + r) * HD + d);
+            const float4 y = *reinterpret_cast<const float4*>(os + ((size_t)w * RT + r) * OS + d);
             L = fmaf(ml[w][1][r], f, L);
             x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
         }
@@ -303,21 +383,17 @@ __global__ void __launch_bounds__(32 * kStepWarps, 3) kv8_attn_step_kernel(Kv8At
 
 template <int HD, typename T>
 cudaError_t launch_kv8_step(const Kv8Attn<T>& a, const Kv8StepPlan& p, cudaStream_t st) {
-    const size_t smem = (size_t)kStepWarps * kStepStages * 32 * HD;
+    constexpr int smem = kStepWarps * StepRing<HD>::kStages * StepRing<HD>::kPageBytes;
+    static_assert(smem >= kStepWarps * 16 * (HD + 4) * 4, "the ring holds the warps' parts");
     const unsigned grid = (unsigned)(p.items * p.splits);
-    static_assert(kStepStages * 32 >= 16 * 4, "the ring holds the warps' parts");
     auto go = [&](auto* kernel, std::atomic<uint32_t>& done) {
-        const cudaError_t e = kv8_smem_once(kernel, (int)smem, p.device, done);
+        const cudaError_t e = kv8_smem_once(kernel, smem, p.device, done);
         if (e != cudaSuccess) return e;
         kernel<<<grid, 32 * kStepWarps, smem, st>>>(a, p);
         return cudaGetLastError();
     };
-    if constexpr (sizeof(T) == 2) {
-        static std::atomic<uint32_t> done16{0};
-        if (!p.pair) return go(&kv8_attn_step_kernel<HD, T, false>, done16);
-    }
-    static std::atomic<uint32_t> done8{0};
-    return go(&kv8_attn_step_kernel<HD, T, true>, done8);
+    static std::atomic<uint32_t> done1{0}, done2{0};
+    return p.tiles == 1 ? go(&kv8_attn_step_kernel<HD, T, 1>, done1) : go(&kv8_attn_step_kernel<HD, T, 2>, done2);
 }
 
 #define POX_KV8_STEP(HD)                                                                                       \

@@ -32,16 +32,15 @@ struct Kv8StepPlan {
     size_t items = 0;
     int device = 0;
     int most_rows = 0x7fffffff;  // sequences of more rows are left to the prompt kernel
-    bool pair = true;  // 8 rows a tile, each as two f16 terms; else 16 rows
+    int tiles = 1;  // of 8 rows each in a CTA
 };
 
-// Rows of a tile: f32 rows, and any rows that fit 8, are carried as pairs of f16 terms.
-inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int G, bool f32, int sms, int most_rows) {
+inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int G, int sms, int most_rows) {
     Kv8StepPlan p;
     p.most_rows = most_rows;
     const long long rows = std::min((long long)b.max_rows * G, (long long)most_rows);
-    p.pair = f32 || rows <= 8;
-    const int rt = p.pair ? 8 : 16;
+    p.tiles = rows <= 8 ? 1 : 2;
+    const int rt = 8 * p.tiles;
     p.row_tiles = (int)((rows + rt - 1) / rt);
     p.items = (size_t)b.seqs * kvh * p.row_tiles;
     const long long pages = (b.max_ctx + kPage - 1) / kPage;
