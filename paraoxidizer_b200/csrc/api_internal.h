@@ -44,12 +44,12 @@ struct pox_tensor {
 
 namespace pox {
 // What the attention over the 8-bit cache keeps for each stream that calls it (calls on different
-// streams may overlap): split partials, and one ticket per item, zero between launches.
+// streams may overlap): the parts of items that are cut, and their tickets, zero between launches.
 struct Kv8Scratch {
     float* part = nullptr;
     size_t part_bytes = 0;
     uint32_t* tickets = nullptr;
-    size_t items = 0;
+    size_t tickets_n = 0;
 };
 }  // namespace pox
 

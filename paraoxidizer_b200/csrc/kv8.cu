@@ -2,7 +2,7 @@
 // appending k and v rows to int8 pages, reading rows back, and the entry points of include/pox_cuda.h
 // (the attention's kernels are in kv8_attn.cu).
 #include <algorithm>
-#include <new>
+#include <exception>
 
 #include "../../include/pox_cuda.h"
 #include "api_internal.h"
@@ -597,28 +597,27 @@ static Kv8Batch batch_view(const pox_kv8_batch* b) {
 
 constexpr int kPromptRows = 64;
 
-// The stream's split partials and tickets for a plan that splits.
+// The stream's places for the parts of items that a plan cuts, and their tickets.
 static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, uint32_t hd, Kv8StepPlan& p) {
-    if (p.splits <= 1) return POX_OK;
-    const size_t need = p.items * p.splits * 8 * p.tiles * (hd + 2) * sizeof(float);
+    const size_t need = p.part_bytes(hd), tickets = (size_t)p.grid;
     try {
         std::lock_guard<std::mutex> lk(ctx->mu);
         Kv8Scratch& k = ctx->kv8[st];
-        if (need > k.part_bytes || p.items > k.items) {
+        if (need > k.part_bytes || tickets > k.tickets_n) {
             cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
             if (cudaStreamIsCapturing(st, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone)
-                return set_error(POX_ERR_INVALID, "split partials must be sized by a call before stream capture");
+                return set_error(POX_ERR_INVALID, "the parts' places must be allocated by a call before stream capture");
             cudaError_t e = cudaStreamSynchronize(st);  // earlier calls may still use the old ones
             if (e != cudaSuccess) return cuda_error(e, "cudaStreamSynchronize");
-            const size_t bytes = std::max(need, k.part_bytes), items = std::max(p.items, k.items);
+            const size_t bytes = std::max(need, k.part_bytes), n = std::max(tickets, k.tickets_n);
             cudaFree(k.part);
             cudaFree(k.tickets);
             k = Kv8Scratch();
             e = cudaMalloc(&k.part, bytes);
-            if (e == cudaSuccess) k.part_bytes = bytes, e = cudaMalloc(&k.tickets, items * sizeof(uint32_t));
-            if (e == cudaSuccess) k.items = items, e = cudaMemsetAsync(k.tickets, 0, items * sizeof(uint32_t), st);
+            if (e == cudaSuccess) k.part_bytes = bytes, e = cudaMalloc(&k.tickets, n * sizeof(uint32_t));
+            if (e == cudaSuccess) k.tickets_n = n, e = cudaMemsetAsync(k.tickets, 0, n * sizeof(uint32_t), st);
             if (e != cudaSuccess) {
-                k.items = 0;  // so that the next call allocates and clears again
+                k.tickets_n = 0;  // so that the next call allocates and clears again
                 return cuda_error(e, "split partials");
             }
         }
@@ -825,8 +824,6 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     const bool step = !prompt || (b->seqs > 1 && b->rows != (unsigned long long)b->seqs * b->max_rows);
     Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, G, ctx->num_sms,
                                      prompt ? kPromptRows : 0x7fffffff);
-    if (plan.items * (unsigned __int128)plan.splits > 0x7fffffffu)
-        return set_error(POX_ERR_UNSUPPORTED, "%zu items of %d splits", plan.items, plan.splits);
     plan.device = ctx->device;
     rc = step ? kv8_scratch(ctx, st, c->head_dim, plan) : POX_OK;
     if (rc) return rc;

@@ -87,7 +87,7 @@ __device__ __forceinline__ bool seq_span(const Kv8Batch& b, uint32_t s, SeqSpan&
     const uint32_t ctx = b.ctx_lens[s];
     o.r0 = r0, o.n = (int)(r1 - r0), o.ctx = (int)ctx;
     if (r1 < r0 || r1 > b.rows || r1 - r0 > b.max_rows || ctx > b.max_ctx) {
-        if ((threadIdx.x & 31) == 0) atomicOr(err, kErrBatch);
+        atomicOr(err, kErrBatch);
         return false;
     }
     return true;

@@ -7,6 +7,7 @@
 // v into the exponent: the products see whole numbers and p <= 2^8, and no page's scale multiplies a tile.
 #include "kv8_attn.h"
 #include "kv8_math.cuh"
+#include "tc05.cuh"
 
 namespace pox {
 
@@ -36,8 +37,12 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {  // an 8 x 8 matrix
     return r;
 }
 
-// One CTA per (sequence, kv head, split of the context, tile of 8 NT rows). Each warp streams whole pages (K and V of
-// 16 tokens of the kv head, 32 HD contiguous bytes) through a ring of its own with one bulk copy a page, and runs both
+// The work of a launch is a line of units: for each sequence in turn, for each kv head and tile of 8 NT rows, kItemUnits
+// for starting on it and one for each page of the sequence. Every CTA takes an equal run of it, whatever the lengths are (with a CTA per split of the longest
+// context, a quarter of the SMs' time went by idle at three sequences of 131k, 116k and 61k tokens). An item that a run cuts leaves its part
+// in the CTA's place (0: of an item begun before, 1: of one that goes on), and the CTA that comes last joins them in order.
+// Within an item each warp streams whole pages (K and V of 16 tokens of the kv head, 32 HD contiguous bytes) through
+// a ring of its own with one bulk copy a page, and runs both
 // products transposed on mma.sync m16n8k16 with f32 accumulators, so that a page is the 16 rows of A and 8 query rows fill N:
 //   S^T (tokens x rows) = K Q^T,   O^T (dims x rows) = V^T P^T.
 // The MMA does not care in which order k and the rows of A run, so they run as the page's bytes lie: lane (g, t) takes
@@ -46,6 +51,12 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {  // an 8 x 8 matrix
 // f32 rows: q and p as two f16 terms each (22 bits), bytes converted exactly. 16-bit rows: q exact, bytes with the
 // offset of bytes_to_f16; p two terms for f16 outputs of up to 8 rows (so that only the output's own rounding
 // remains), one for bf16 and for more rows (2^-11 of p).
+constexpr uint32_t kWholePages = 128;
+
+__device__ __forceinline__ unsigned long long div_u64(unsigned long long a, uint32_t b) {
+    return a >> 32 ? a / b : (uint32_t)a / b;  // (the long division is a hundred instructions)
+}
+
 template <int HD, typename T, int NT>
 __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_step_kernel(Kv8Attn<T> a, Kv8StepPlan p) {
     constexpr bool F32 = sizeof(T) == 4, PLO = F32 || (std::is_same<T, __half>::value && NT == 1);
@@ -56,328 +67,412 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
     __shared__ float ml[kStepWarps][2][RT];
     __shared__ uint32_t last_cta;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    uint32_t bi = blockIdx.x;
-    const int rt = bi % p.row_tiles;
-    bi /= p.row_tiles;
-    const int sp = bi % p.splits;
-    bi /= p.splits;
-    const int h = bi % a.c.kvh;
-    const uint32_t s = bi / a.c.kvh;
-    SeqSpan sq;
-    if (!seq_span(a.b, s, sq, a.err)) return;
-    const int rows = sq.n * a.G, row0 = rt * RT;
-    if (row0 >= rows || rows > p.most_rows) return;
-    const int pos0 = sq.ctx - sq.n, pmin = pos0 + row0 / a.G, pmax = pos0 + (min(row0 + RT, rows) - 1) / a.G;
-    const int pages = pmax < 0 ? 0 : pmax / kPage + 1;
-    const int ns = max(1, (pages + p.pages_per_split - 1) / p.pages_per_split);
-    if (sp >= ns) return;
-
-    // this warp's pages: first, first + W, ..; lane i holds the i-th one's place and scales
-    const int first = sp * p.pages_per_split + warp, end = min(pages, (sp + 1) * p.pages_per_split);
-    const int cnt = first < end ? (end - first + kStepWarps - 1) / kStepWarps : 0;
     const uint32_t ring = smem_u32(smem) + warp * NST * PB, bar = smem_u32(&bars[warp][0]);
     if (lane == 0) {
         for (int i = 0; i < NST; i++) mbar_init(bar + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    size_t place = 0;
-    bool there = false;
-    if (lane < cnt) {
-        const int blk = a.b.btab[(size_t)s * a.b.mbps + first + lane * kStepWarps];
-        there = blk >= 0 && (uint32_t)blk < a.c.num_blocks;
-        if (!there) atomicOr(a.err, kErrAttnPage);
-        place = there ? (size_t)blk * a.c.kvh + h : 0;
-    }
-    const unsigned there_m = __ballot_sync(0xffffffffu, there);
-    auto fetch = [&](int i, int st) {  // page i of this warp into its stage (a page out of range: page 0, unread)
-        const size_t pl = __shfl_sync(0xffffffffu, (unsigned long long)place, i);
-        if (lane == 0) {
-            mbar_expect_tx(bar + 8 * st, PB);
-            bulk_g2s(ring + st * PB, a.c.pages + pl * PB, PB, bar + 8 * st);
-        }
+    // units of a sequence (one item at least, so that rows that see nothing are written), and where this CTA's run begins
+    auto units = [&](uint32_t s, SeqSpan& q) -> unsigned long long {
+        if (!seq_span(a.b, s, q, a.err)) return 0;
+        const int rows = q.n * a.G;
+        if (rows > p.most_rows) return 0;
+        return (unsigned long long)a.c.kvh * ((rows + RT - 1) / RT) * (kItemUnits + max((q.ctx + kPage - 1) / kPage, 1));
     };
-    for (int i = 0; i < min(cnt, NST); i++) fetch(i, i);
-    const float2 ab = lane < cnt ? *reinterpret_cast<const float2*>(a.c.scales + place * 2) : make_float2(0.f, 0.f);
-    // log2 b; a scale of 0 stands for zeros whatever the bytes: 1e-30 of them is nothing next to any other page
-    const float lb = log2f(fmaxf(ab.y, 1e-30f) + (ab.y - ab.y)), ib = 1.0f / fmaxf(ab.y, 1e-30f);
-
-    // B fragments of the rows: lane (g, t) the dims of row g that t takes of a token. Then, for the rows 2 t and 2 t + 1 that
-    // this lane's scores belong to: what takes a product to a score, its offset, and the last position seen
-    uint32_t qb[NT][F32 ? 2 : 1][KW][2];
-    float qf[NT][2], qo[NT][2];
-    int rpos[NT][2];
+    unsigned long long total = 0;
+    for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32) {
+        SeqSpan q;
+        total += s0 + lane < a.b.seqs ? units(s0 + lane, q) : 0;
+    }
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int row = row0 + 8 * n + g;
-        const bool ok = row < rows;
-        const T* q = a.q.at((size_t)sq.r0 + (ok ? row / a.G : 0), h * a.G + (ok ? row % a.G : 0));
-        float v[KW][4], m = 0.f;
+    for (int k = 16; k; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
+    const uint32_t run = max((uint32_t)div_u64(total + gridDim.x - 1, gridDim.x), (uint32_t)p.min_units);
+    // An item of up to `whole` pages is not cut (joining costs about what 64 pages do), and none within `edge` of its
+    // ends: the border goes to the nearer end.
+    const uint32_t whole = min(kWholePages, 2 * run), edge = min(16u, run / 2);
+    auto border = [&](uint32_t u, uint32_t all) {  // a border u units into an item of `all`
+        if (all - kItemUnits <= whole) return 2 * u < all ? 0u : all;
+        return u < kItemUnits + edge ? 0u : u > all - edge ? all : u;
+    };
+    const unsigned long long x_begin = (unsigned long long)run * blockIdx.x, x_end = x_begin + run;
+    if (x_begin >= total) return;
+    uint32_t s = 0;
+    unsigned long long base = 0;  // the line's place where sequence s begins
+    for (uint32_t s0 = 0;; s0 += 32) {
+        SeqSpan q;
+        unsigned long long u = s0 + lane < a.b.seqs ? units(s0 + lane, q) : 0, sum = u;
 #pragma unroll
-        for (int w = 0; w < KW; w++) {
-            const int d = HD == 32 ? 8 * t + 4 * w : 64 * (w / 4) + 16 * t + 4 * (w % 4);
-            if (ok) load4(q + d, a.vec, v[w]);
-            else v[w][0] = v[w][1] = v[w][2] = v[w][3] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(v[w][i]));
+        for (int k = 1; k < 32; k *= 2) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, sum, k);
+            if (lane >= k) sum += y;
         }
-        float f = 1.f, inv = 1.f, sum = 0.f;
-        if constexpr (!std::is_same<T, __half>::value) {
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            f = row_factor(m, inv);
+        const unsigned m = __ballot_sync(0xffffffffu, base + sum > x_begin);
+        if (m) {
+            s = s0 + __ffs(m) - 1;
+            base += __shfl_sync(0xffffffffu, sum - u, __ffs(m) - 1);
+            break;
         }
-#pragma unroll
-        for (int w = 0; w < KW; w++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float x = v[w][2 * i] * f, y = v[w][2 * i + 1] * f;
-                qb[n][0][w][i] = pack_f16(x, y);
-                if constexpr (F32) {
-                    const float2 hi = unpack_f16(qb[n][0][w][i]);
-                    qb[n][F32][w][i] = pack_f16(x - hi.x, y - hi.y);
-                } else {
-                    sum += x + y;  // (16-bit rows are f16 exactly)
-                }
-            }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            qf[n][e] = __shfl_sync(0xffffffffu, inv, 8 * t + 4 * e) * a.scale * (F32 ? 1.0f : 16777216.0f);
-            qo[n][e] = F32 ? 0.f : -kOffset * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
-            const int r = row0 + 8 * n + 2 * t + e;
-            rpos[n][e] = r < rows ? pos0 + r / a.G : 0;
-        }
+        base += __shfl_sync(0xffffffffu, sum, 31);
     }
 
-    float o[NT][NJ][4], m[NT][2], l[NT][2], ps[NT][2];  // ps: the sum of p as the product sees it
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 2; e++) m[n][e] = -INFINITY, l[n][e] = 0.f, ps[n][e] = 0.f;
-    }
-    const int tok = 4 * (g >> 1) + (g & 1);
     bool bad = false;
     int st = 0, ph = 0;
-    for (int i = 0; i < cnt; i++) {
-        const int page = first + i * kStepWarps;
-        const uint32_t base = ring + st * PB;
-        bad = __any_sync(0xffffffffu, !mbar_wait(bar + 8 * st, ph));
-        const float pa = __shfl_sync(0xffffffffu, ab.x, i), pl = __shfl_sync(0xffffffffu, lb, i),
-                    pi = __shfl_sync(0xffffffffu, ib, i);
-        // S^T: tokens tok (rows g of A) and tok + 2 (rows g + 8); two chains of products
-        float sc[NT][2][4];
+    SeqSpan sq;
+    unsigned long long su = units(s, sq);
+    uint32_t all = kItemUnits + max((sq.ctx + kPage - 1) / kPage, 1);
+    uint32_t item = (uint32_t)div_u64(x_begin - base, all);
+    uint32_t u0 = border((uint32_t)(x_begin - base - (unsigned long long)item * all), all);  // of the item, this CTA's first unit
+    for (;; item++, u0 = 0) {  // the items of this CTA's run
+        unsigned long long x0 = base + (unsigned long long)item * all;  // where the item begins
+        while (x0 >= base + su) {  // the sequence is done
+            base += su;
+            if (x0 >= total || base >= x_end) return;
+            su = units(++s, sq);
+            all = kItemUnits + max((sq.ctx + kPage - 1) / kPage, 1);
+            item = 0, x0 = base;
+        }
+        if (x0 >= x_end) return;
+        const uint32_t u1 = x0 + all <= x_end ? all : border((uint32_t)(x_end - x0), all);
+        if (u0 >= u1) continue;
+        const int rows = sq.n * a.G, tiles = (rows + RT - 1) / RT;
+        // tiles of a sequence in the order first, last, second, ..: early ones see fewer pages of a chunk
+        const int h = item / tiles, k_rt = item % tiles, rt = k_rt & 1 ? tiles - 1 - k_rt / 2 : k_rt / 2, row0 = rt * RT;
+        const int pos0 = sq.ctx - sq.n, pmin = pos0 + row0 / a.G, pmax = pos0 + (min(row0 + RT, rows) - 1) / a.G;
+        const int pages = pmax < 0 ? 0 : pmax / kPage + 1;
+        const int page0 = max((int)u0 - kItemUnits, 0), page1 = min(pages, (int)u1 - kItemUnits);
+        // the CTA that holds the item's first part, and the parts: one more than the borders that cut it
+        uint32_t c0 = blockIdx.x, ns = 1;
+        if (u0 > 0 || u1 < all) {
+            const uint32_t i0 = (uint32_t)div_u64(x0 + kItemUnits + edge + run - 1, run), i1 = (uint32_t)div_u64(x0 + all - edge, run);
+            c0 = i0 - 1, ns = i1 - i0 + 2;
+        }
+
+        // this warp's pages: first, first + W, ..; lane i holds place and scales of the i-th of 32, and of the next 32
+        const int first = page0 + warp, cnt = first < page1 && !bad ? (page1 - first + kStepWarps - 1) / kStepWarps : 0;
+        struct Entry {
+            size_t place;
+            float2 ab;
+            unsigned there;
+        } cur, nxt;
+        auto entries = [&](int i0) {
+            Entry e{0, make_float2(0.f, 0.f), 0};
+            bool there = false;
+            if (i0 + lane < cnt) {
+                const int blk = a.b.btab[(size_t)s * a.b.mbps + first + (i0 + lane) * kStepWarps];
+                there = blk >= 0 && (uint32_t)blk < a.c.num_blocks;
+                if (!there) atomicOr(a.err, kErrAttnPage);
+                e.place = there ? (size_t)blk * a.c.kvh + h : 0;
+            }
+            e.there = __ballot_sync(0xffffffffu, there);
+            return e;
+        };
+        auto scales = [&](Entry& e, int i0) {
+            if (i0 + lane < cnt) e.ab = *reinterpret_cast<const float2*>(a.c.scales + e.place * 2);
+        };
+        // log2 b; a scale of 0 stands for zeros whatever the bytes: 1e-30 of them is nothing next to any other page
+        float lb, ib;
+        auto logs = [&](const Entry& e) {
+            lb = log2f(fmaxf(e.ab.y, 1e-30f) + (e.ab.y - e.ab.y)), ib = 1.0f / fmaxf(e.ab.y, 1e-30f);
+        };
+        auto fetch = [&](const Entry& e, int i, int st) {  // page i of this warp into its stage (one out of range: page 0, unread)
+            const size_t pl = __shfl_sync(0xffffffffu, (unsigned long long)e.place, i & 31);
+            if (lane == 0) {
+                mbar_expect_tx(bar + 8 * st, PB);
+                bulk_g2s(ring + st * PB, a.c.pages + pl * PB, PB, bar + 8 * st);
+            }
+        };
+        cur = entries(0);
+        for (int i = 0, k = st; i < min(cnt, NST); i++) {
+            fetch(cur, i, k);
+            if (++k == NST) k = 0;
+        }
+        scales(cur, 0);
+        logs(cur);
+
+        // B fragments of the rows: lane (g, t) the dims of row g that t takes of a token. Then, for the rows 2 t and 2 t + 1 that
+        // this lane's scores belong to: what takes a product to a score, its offset, and the last position seen
+        uint32_t qb[NT][F32 ? 2 : 1][KW][2];
+        float qf[NT][2], qo[NT][2];
+        int rpos[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT; n++) {
+            const int row = row0 + 8 * n + g;
+            const bool ok = row < rows;
+            const T* q = a.q.at((size_t)sq.r0 + (ok ? row / a.G : 0), h * a.G + (ok ? row % a.G : 0));
+            float v[KW][4], m = 0.f;
 #pragma unroll
-            for (int k = 0; k < 2; k++)
+            for (int w = 0; w < KW; w++) {
+                const int d = HD == 32 ? 8 * t + 4 * w : 64 * (w / 4) + 16 * t + 4 * (w % 4);
+                if (ok) load4(q + d, a.vec, v[w]);
+                else v[w][0] = v[w][1] = v[w][2] = v[w][3] = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) sc[n][k][e] = k == 0 ? qo[n][e & 1] : 0.f;
-        uint32_t kw[2][KW];
+                for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(v[w][i]));
+            }
+            float f = 1.f, inv = 1.f, sum = 0.f;
+            if constexpr (!std::is_same<T, __half>::value) {
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                f = row_factor(m, inv);
+            }
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const uint32_t at = base + (tok + 2 * u) * HD;
-            if constexpr (HD == 32) {
-                const uint2 x = lds64(at + 8 * t);
-                kw[u][0] = x.x, kw[u][1] = x.y;
-            } else {
+            for (int w = 0; w < KW; w++)
 #pragma unroll
-                for (int c = 0; c < HD / 64; c++) {
-                    const uint4 x = lds128(at + (HD == 128 ? (64 * c + 16 * t) ^ ((g & 1) << 6) : 16 * t));
-                    kw[u][4 * c] = x.x, kw[u][4 * c + 1] = x.y, kw[u][4 * c + 2] = x.z, kw[u][4 * c + 3] = x.w;
+                for (int i = 0; i < 2; i++) {
+                    const float x = v[w][2 * i] * f, y = v[w][2 * i + 1] * f;
+                    qb[n][0][w][i] = pack_f16(x, y);
+                    if constexpr (F32) {
+                        const float2 hi = unpack_f16(qb[n][0][w][i]);
+                        qb[n][F32][w][i] = pack_f16(x - hi.x, y - hi.y);
+                    } else {
+                        sum += x + y;  // (16-bit rows are f16 exactly)
+                    }
                 }
-            }
-        }
-#pragma unroll
-        for (int w = 0; w < KW; w++) {
-            uint32_t a0, a1, a2, a3;
-            bytes_to_f16<F32>(kw[0][w], a0, a2);
-            bytes_to_f16<F32>(kw[1][w], a1, a3);
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                mma_16816(sc[n][w & 1], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1]);
-                if constexpr (F32) mma_16816(sc[n][w & 1], a0, a1, a2, a3, qb[n][F32][w][0], qb[n][F32][w][1]);
-            }
-        }
-        // u of tokens tok, tok + 2 and rows 2 t, 2 t + 1
-        const bool seen = there_m >> i & 1, whole = page * kPage + kPage - 1 <= pmin && seen;
-        float u[NT][4];
-        bool grow = false;
-#pragma unroll
-        for (int n = 0; n < NT; n++)
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float f = qf[n][e] * pa;
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    float x = fmaf(sc[n][0][2 * k + e] + sc[n][1][2 * k + e], f, pl);
-                    if (!whole && (page * kPage + tok + 2 * k > rpos[n][e] || !seen)) x = -INFINITY;
-                    u[n][2 * k + e] = x;
-                }
-                grow |= fmaxf(u[n][e], u[n][2 + e]) > m[n][e] + 8.0f;
+                qf[n][e] = __shfl_sync(0xffffffffu, inv, 8 * t + 4 * e) * a.scale * (F32 ? 1.0f : 16777216.0f);
+                qo[n][e] = F32 ? 0.f : -kOffset * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
+                const int r = row0 + 8 * n + 2 * t + e;
+                rpos[n][e] = r < rows ? pos0 + r / a.G : 0;
             }
-        // the reference moves only when p would pass 2^8: after the first pages it hardly ever does
-        if (__any_sync(0xffffffffu, grow)) {
+        }
+
+        float o[NT][NJ][4], m[NT][2], l[NT][2], ps[NT][2];  // ps: the sum of p as the product sees it
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; e++) m[n][e] = -INFINITY, l[n][e] = 0.f, ps[n][e] = 0.f;
+        }
+        const int tok = 4 * (g >> 1) + (g & 1);
+        for (int i = 0; i < cnt; i++) {
+            const int page = first + i * kStepWarps;
+            if ((i & 31) == 0) {
+                if (i) cur = nxt, logs(cur);
+                nxt = entries(i + 32);
+                scales(nxt, i + 32);
+            }
+            const uint32_t base = ring + st * PB;
+            bad = __any_sync(0xffffffffu, !mbar_wait(bar + 8 * st, ph));
+            const float pa = __shfl_sync(0xffffffffu, cur.ab.x, i & 31), pl = __shfl_sync(0xffffffffu, lb, i & 31),
+                        pi = __shfl_sync(0xffffffffu, ib, i & 31);
+            // S^T: tokens tok (rows g of A) and tok + 2 (rows g + 8); two chains of products
+            float sc[NT][2][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[n][k][e] = k == 0 ? qo[n][e & 1] : 0.f;
+            uint32_t kw[2][KW];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const uint32_t at = base + (tok + 2 * u) * HD;
+                if constexpr (HD == 32) {
+                    const uint2 x = lds64(at + 8 * t);
+                    kw[u][0] = x.x, kw[u][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < HD / 64; c++) {
+                        const uint4 x = lds128(at + (HD == 128 ? (64 * c + 16 * t) ^ ((g & 1) << 6) : 16 * t));
+                        kw[u][4 * c] = x.x, kw[u][4 * c + 1] = x.y, kw[u][4 * c + 2] = x.z, kw[u][4 * c + 3] = x.w;
+                    }
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < KW; w++) {
+                uint32_t a0, a1, a2, a3;
+                bytes_to_f16<F32>(kw[0][w], a0, a2);
+                bytes_to_f16<F32>(kw[1][w], a1, a3);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    mma_16816(sc[n][w & 1], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1]);
+                    if constexpr (F32) mma_16816(sc[n][w & 1], a0, a1, a2, a3, qb[n][F32][w][0], qb[n][F32][w][1]);
+                }
+            }
+            // u of tokens tok, tok + 2 and rows 2 t, 2 t + 1
+            const bool seen = cur.there >> (i & 31) & 1, whole = page * kPage + kPage - 1 <= pmin && seen;
+            float u[NT][4];
+            bool grow = false;
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float to = fmaxf(u[n][e], u[n][2 + e]);
+                    const float f = qf[n][e] * pa;
 #pragma unroll
-                    for (int k = 4; k < 32; k *= 2) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, k));
-                    to = to > m[n][e] + 8.0f ? to : m[n][e];
-                    const float f = m[n][e] == -INFINITY ? (to == -INFINITY ? 1.f : 0.f) : ex2(m[n][e] - to);
-                    m[n][e] = to;
-                    l[n][e] *= f, ps[n][e] *= f;
-#pragma unroll
-                    for (int j = 0; j < NJ; j++) o[n][j][e] *= f, o[n][j][2 + e] *= f;
+                    for (int k = 0; k < 2; k++) {
+                        float x = fmaf(sc[n][0][2 * k + e] + sc[n][1][2 * k + e], f, pl);
+                        if (!whole && (page * kPage + tok + 2 * k > rpos[n][e] || !seen)) x = -INFINITY;
+                        u[n][2 * k + e] = x;
+                    }
+                    grow |= fmaxf(u[n][e], u[n][2 + e]) > m[n][e] + 8.0f;
                 }
-        }
-        uint32_t pb[NT][PLO ? 2 : 1][2];  // B fragments of P^T: tokens 4 t, 4 t + 1 | 4 t + 2, 4 t + 3 of row g
+            // the reference moves only when p would pass 2^8: after the first pages it hardly ever does
+            if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            float x[4], y[2] = {0.f, 0.f};
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = ex2(u[n][e] - (m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1]));
+                    for (int e = 0; e < 2; e++) {
+                        float to = fmaxf(u[n][e], u[n][2 + e]);
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const uint32_t hi = pack_f16(x[2 * k], x[2 * k + 1]);
-                const float2 r = unpack_f16(hi);
-                pb[n][0][k] = transpose8(hi);
-                if constexpr (PLO) {
-                    const uint32_t lo = pack_f16(x[2 * k] - r.x, x[2 * k + 1] - r.y);
-                    pb[n][PLO][k] = transpose8(lo);
-                    y[0] += x[2 * k], y[1] += x[2 * k + 1];
-                } else {
-                    y[0] += r.x, y[1] += r.y;
-                }
+                        for (int k = 4; k < 32; k *= 2) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, k));
+                        to = to > m[n][e] + 8.0f ? to : m[n][e];
+                        const float f = m[n][e] == -INFINITY ? (to == -INFINITY ? 1.f : 0.f) : ex2(m[n][e] - to);
+                        m[n][e] = to;
+                        l[n][e] *= f, ps[n][e] *= f;
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) o[n][j][e] *= f, o[n][j][2 + e] *= f;
+                    }
             }
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                if (y[e] != 0.f) l[n][e] = fmaf(y[e], pi, l[n][e]);  // (an unseen page's scale may be anything)
-                if (!F32) ps[n][e] += y[e];
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            uint32_t w0, w1, a0, a1, a2, a3;
-            const uint32_t at = base + kPage * HD + (16 * j + g) * kPage + 4 * t;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0) : "r"(at));
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1) : "r"(at + 8 * kPage));
-            bytes_to_f16<F32>(w0, a0, a2);
-            bytes_to_f16<F32>(w1, a1, a3);
+            uint32_t pb[NT][PLO ? 2 : 1][2];  // B fragments of P^T: tokens 4 t, 4 t + 1 | 4 t + 2, 4 t + 3 of row g
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                mma_16816(o[n][j], a0, a1, a2, a3, pb[n][0][0], pb[n][0][1]);
-                if constexpr (PLO) mma_16816(o[n][j], a0, a1, a2, a3, pb[n][PLO][0], pb[n][PLO][1]);
+                float x[4], y[2] = {0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = ex2(u[n][e] - (m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1]));
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t hi = pack_f16(x[2 * k], x[2 * k + 1]);
+                    const float2 r = unpack_f16(hi);
+                    pb[n][0][k] = transpose8(hi);
+                    if constexpr (PLO) {
+                        const uint32_t lo = pack_f16(x[2 * k] - r.x, x[2 * k + 1] - r.y);
+                        pb[n][PLO][k] = transpose8(lo);
+                        y[0] += x[2 * k], y[1] += x[2 * k + 1];
+                    } else {
+                        y[0] += r.x, y[1] += r.y;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    if (y[e] != 0.f) l[n][e] = fmaf(y[e], pi, l[n][e]);  // (an unseen page's scale may be anything)
+                    if (!F32) ps[n][e] += y[e];
+                }
             }
-        }
-        __syncwarp();  // every lane has read the stage
-        if (bad) {  // a copy did not come in time: give the ones in flight as long again, and leave
-            for (int k = i; k < min(cnt, i + NST); k++) {
-                mbar_wait(bar + 8 * st, ph);
-                if (++st == NST) st = 0, ph ^= 1;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                uint32_t w0, w1, a0, a1, a2, a3;
+                const uint32_t at = base + kPage * HD + (16 * j + g) * kPage + 4 * t;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0) : "r"(at));
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1) : "r"(at + 8 * kPage));
+                bytes_to_f16<F32>(w0, a0, a2);
+                bytes_to_f16<F32>(w1, a1, a3);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    mma_16816(o[n][j], a0, a1, a2, a3, pb[n][0][0], pb[n][0][1]);
+                    if constexpr (PLO) mma_16816(o[n][j], a0, a1, a2, a3, pb[n][PLO][0], pb[n][PLO][1]);
+                }
             }
-            if (lane == 0) atomicOr(a.err, kErrWaitRing);
-            break;
+            __syncwarp();  // every lane has read the stage
+            if (bad) {  // a copy did not come in time: give the ones in flight as long again, and leave
+                for (int k = i; k < min(cnt, i + NST); k++) {
+                    mbar_wait(bar + 8 * st, ph);
+                    if (++st == NST) st = 0, ph ^= 1;
+                }
+                if (lane == 0) atomicOr(a.err, kErrWaitRing);
+                break;
+            }
+            if (i + NST < cnt) fetch(((i + NST) ^ i) & ~31 ? nxt : cur, i + NST, st);
+            if (++st == NST) st = 0, ph ^= 1;
         }
-        if (i + NST < cnt) fetch(i + NST, st);
-        if (++st == NST) st = 0, ph ^= 1;
-    }
 
-    // the warps' parts: (m, l) and o in units of 2^m, through the ring's space
-    constexpr int OS = HD + 4;  // floats of a row there (rows 2 t of a warp's stores in distinct banks)
-    float off[NT][2];
+        // the warps' parts: (m, l) and o in units of 2^m, through the ring's space
+        constexpr int OS = HD + 4;  // floats of a row there (rows 2 t of a warp's stores in distinct banks)
+        float off[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            float y = l[n][e], z = ps[n][e];
+            for (int e = 0; e < 2; e++) {
+                float y = l[n][e], z = ps[n][e];
 #pragma unroll
-            for (int k = 4; k < 32; k *= 2) {
-                y += __shfl_xor_sync(0xffffffffu, y, k);
-                if (!F32) z += __shfl_xor_sync(0xffffffffu, z, k);
+                for (int k = 4; k < 32; k *= 2) {
+                    y += __shfl_xor_sync(0xffffffffu, y, k);
+                    if (!F32) z += __shfl_xor_sync(0xffffffffu, z, k);
+                }
+                if (g == 0) ml[warp][0][8 * n + 2 * t + e] = m[n][e], ml[warp][1][8 * n + 2 * t + e] = y;
+                off[n][e] = -128.0f * z;
             }
-            if (g == 0) ml[warp][0][8 * n + 2 * t + e] = m[n][e], ml[warp][1][8 * n + 2 * t + e] = y;
-            off[n][e] = -128.0f * z;
+        __syncthreads();
+        float* os = reinterpret_cast<float*>(smem);  // [warp][RT][OS]
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    os[((size_t)warp * RT + 8 * n + 2 * t + (e & 1)) * OS + 16 * j + 8 * (e >> 1) + g] =
+                        F32 ? o[n][j][e] : fmaf(o[n][j][e], 16777216.0f, off[n][e & 1]);
+        __syncthreads();
+        float* part = p.part + (size_t)(2 * blockIdx.x + (blockIdx.x == c0)) * RT * (HD + 2);
+        const int valid = min(RT, rows - row0);
+        for (int i = tid; i < valid * (HD / 4); i += 32 * kStepWarps) {
+            const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int w = 0; w < kStepWarps; w++) M = fmaxf(M, ml[w][0][r]);
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kStepWarps; w++) {
+                // NaN scores leave m at -inf with l NaN: the weight of such a part is 1, so that the row is NaN
+                const float f = ml[w][0][r] == -INFINITY ? (ml[w][1][r] == 0.f ? 0.f : 1.f) : ex2(ml[w][0][r] - M);
+                const float4 y = *reinterpret_cast<const float4*>(os + ((size_t)w * RT + r) * OS + d);
+                L = fmaf(ml[w][1][r], f, L);
+                x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+            }
+            if (ns == 1) {
+                const float inv = L == 0.f ? 0.f : 1.0f / L;
+                const int row = row0 + r;
+                store4(a.out.at((size_t)sq.r0 + row / a.G, h * a.G + row % a.G) + d, a.vec,
+                       make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+            } else {
+                float* y = part + (size_t)r * (HD + 2);
+                *reinterpret_cast<float2*>(y + 2 + d) = make_float2(x.x, x.y);
+                *reinterpret_cast<float2*>(y + 4 + d) = make_float2(x.z, x.w);
+                if (d == 0) *reinterpret_cast<float2*>(y) = make_float2(M, L);
+            }
         }
-    __syncthreads();
-    float* os = reinterpret_cast<float*>(smem);  // [warp][RT][OS]
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                os[((size_t)warp * RT + 8 * n + 2 * t + (e & 1)) * OS + 16 * j + 8 * (e >> 1) + g] =
-                    F32 ? o[n][j][e] : fmaf(o[n][j][e], 16777216.0f, off[n][e & 1]);
-    __syncthreads();
-    const size_t item = ((size_t)s * a.c.kvh + h) * p.row_tiles + rt;
-    float* part = p.part + (item * p.splits + sp) * RT * (HD + 2);
-    const int valid = min(RT, rows - row0);
-    for (int i = tid; i < valid * (HD / 4); i += 32 * kStepWarps) {
-        const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < kStepWarps; w++) M = fmaxf(M, ml[w][0][r]);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kStepWarps; w++) {
-            // NaN scores leave m at -inf with l NaN: the weight of such a part is 1, so that the row is NaN
-            const float f = ml[w][0][r] == -INFINITY ? (ml[w][1][r] == 0.f ? 0.f : 1.f) : ex2(ml[w][0][r] - M);
-            const float4 y = *reinterpret_cast<const float4*>(os + ((size_t)w * RT + r) * OS + d);
-            L = fmaf(ml[w][1][r], f, L);
-            x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+        bool last = false;
+        if (ns > 1) {  // the CTA that comes last joins all parts, in their order
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                last_cta = atomicAdd(p.tickets + c0, 1u) == ns - 1;
+                if (last_cta) p.tickets[c0] = 0;
+            }
+            __syncthreads();
+            last = last_cta;
         }
-        if (ns == 1) {
+        if (last) {
+            __threadfence();
+        for (int i = tid; i < valid * (HD / 4); i += 32 * kStepWarps) {
+            const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
+            float M = -INFINITY, L = 0.f;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (uint32_t k = 0; k < ns; k++) {
+                const float* y = p.part + ((size_t)(2 * (c0 + k) + (k == 0)) * RT + r) * (HD + 2);
+                const float2 w = __ldcg(reinterpret_cast<const float2*>(y));
+                const float2 u = __ldcg(reinterpret_cast<const float2*>(y + 2 + d)),
+                             v = __ldcg(reinterpret_cast<const float2*>(y + 4 + d));
+                const float to = fmaxf(M, w.x);
+                const float fo = M == -INFINITY ? (L == 0.f ? 0.f : 1.f) : ex2(M - to),
+                            fn = w.x == -INFINITY ? (w.y == 0.f ? 0.f : 1.f) : ex2(w.x - to);
+                M = to;
+                L = fmaf(L, fo, w.y * fn);
+                x.x = fmaf(x.x, fo, u.x * fn), x.y = fmaf(x.y, fo, u.y * fn);
+                x.z = fmaf(x.z, fo, v.x * fn), x.w = fmaf(x.w, fo, v.y * fn);
+            }
             const float inv = L == 0.f ? 0.f : 1.0f / L;
             const int row = row0 + r;
             store4(a.out.at((size_t)sq.r0 + row / a.G, h * a.G + row % a.G) + d, a.vec,
                    make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-        } else {
-            float* y = part + (size_t)r * (HD + 2);
-            *reinterpret_cast<float2*>(y + 2 + d) = make_float2(x.x, x.y);
-            *reinterpret_cast<float2*>(y + 4 + d) = make_float2(x.z, x.w);
-            if (d == 0) *reinterpret_cast<float2*>(y) = make_float2(M, L);
         }
-    }
-    if (ns == 1) return;
-    // the split that arrives last joins them all, in their order
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        last_cta = atomicAdd(p.tickets + item, 1u) == (uint32_t)ns - 1;
-        if (last_cta) p.tickets[item] = 0;
-    }
-    __syncthreads();
-    if (!last_cta) return;
-    __threadfence();
-    const float* all = p.part + item * p.splits * RT * (HD + 2);
-    for (int i = tid; i < valid * (HD / 4); i += 32 * kStepWarps) {
-        const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
-        float M = -INFINITY, L = 0.f;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int k = 0; k < ns; k++) {
-            const float* y = all + ((size_t)k * RT + r) * (HD + 2);
-            const float2 w = __ldcg(reinterpret_cast<const float2*>(y));
-            const float2 u = __ldcg(reinterpret_cast<const float2*>(y + 2 + d)),
-                         v = __ldcg(reinterpret_cast<const float2*>(y + 4 + d));
-            const float to = fmaxf(M, w.x);
-            const float fo = M == -INFINITY ? (L == 0.f ? 0.f : 1.f) : ex2(M - to),
-                        fn = w.x == -INFINITY ? (w.y == 0.f ? 0.f : 1.f) : ex2(w.x - to);
-            M = to;
-            L = fmaf(L, fo, w.y * fn);
-            x.x = fmaf(x.x, fo, u.x * fn), x.y = fmaf(x.y, fo, u.y * fn);
-            x.z = fmaf(x.z, fo, v.x * fn), x.w = fmaf(x.w, fo, v.y * fn);
         }
-        const float inv = L == 0.f ? 0.f : 1.0f / L;
-        const int row = row0 + r;
-        store4(a.out.at((size_t)sq.r0 + row / a.G, h * a.G + row % a.G) + d, a.vec,
-               make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+        fence_proxy_async_smem();  // the ring's space goes back to the copies
+        __syncthreads();
     }
 }
 
@@ -385,11 +480,10 @@ template <int HD, typename T>
 cudaError_t launch_kv8_step(const Kv8Attn<T>& a, const Kv8StepPlan& p, cudaStream_t st) {
     constexpr int smem = kStepWarps * StepRing<HD>::kStages * StepRing<HD>::kPageBytes;
     static_assert(smem >= kStepWarps * 16 * (HD + 4) * 4, "the ring holds the warps' parts");
-    const unsigned grid = (unsigned)(p.items * p.splits);
     auto go = [&](auto* kernel, std::atomic<uint32_t>& done) {
         const cudaError_t e = kv8_smem_once(kernel, smem, p.device, done);
         if (e != cudaSuccess) return e;
-        kernel<<<grid, 32 * kStepWarps, smem, st>>>(a, p);
+        kernel<<<p.grid, 32 * kStepWarps, smem, st>>>(a, p);
         return cudaGetLastError();
     };
     static std::atomic<uint32_t> done1{0}, done2{0};

@@ -9,8 +9,8 @@
 
 namespace pox {
 
-constexpr int kStepWarps = 4;        // warps of a CTA of the step kernel
-constexpr int kStepMostPages = 128;  // pages of a split: one lane of a warp holds the entry of each of its pages
+constexpr int kStepWarps = 4;   // warps of a CTA of the step kernel
+constexpr int kItemUnits = 32;  // what an item of it costs besides its pages, in pages (eight rounds of the warps)
 
 template <typename T>
 struct Kv8Attn {
@@ -24,15 +24,16 @@ struct Kv8Attn {
     int* err;
 };
 
-// How the step kernel splits its work: row tiles of a (sequence, kv head) pair and splits of the context.
+// How the step kernel divides its work (see there).
 struct Kv8StepPlan {
-    int row_tiles = 1, splits = 1, pages_per_split = kStepMostPages;
-    float* part = nullptr;        // [items][splits][rows of a tile][hd + 2] when splits > 1
-    uint32_t* tickets = nullptr;  // [items], zero between launches
-    size_t items = 0;
-    int device = 0;
+    int tiles = 1;      // of 8 rows each in an item
+    int grid = 1;       // CTAs, each with an equal run of units (pages of an item)
+    int min_units = 1;  // of a run
     int most_rows = 0x7fffffff;  // sequences of more rows are left to the prompt kernel
-    int tiles = 1;  // of 8 rows each in a CTA
+    int device = 0;
+    float* part = nullptr;        // [grid][2][8 tiles][hd + 2]
+    uint32_t* tickets = nullptr;  // [grid], zero between launches
+    size_t part_bytes(uint32_t hd) const { return (size_t)grid * 2 * 8 * tiles * (hd + 2) * sizeof(float); }
 };
 
 inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int G, int sms, int most_rows) {
@@ -40,16 +41,12 @@ inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int G, int sms, int
     p.most_rows = most_rows;
     const long long rows = std::min((long long)b.max_rows * G, (long long)most_rows);
     p.tiles = rows <= 8 ? 1 : 2;
-    const int rt = 8 * p.tiles;
-    p.row_tiles = (int)((rows + rt - 1) / rt);
-    p.items = (size_t)b.seqs * kvh * p.row_tiles;
-    const long long pages = (b.max_ctx + kPage - 1) / kPage;
-    // about four CTAs for each of the three places that an SM has, but two pages at least for each warp
-    long long pps = (long long)(p.items * (double)pages / (12.0 * sms));
-    pps = std::min<long long>(kStepMostPages, std::max<long long>(pps, 2 * kStepWarps));
-    p.splits = (int)std::max<long long>(1, (pages + pps - 1) / pps);
-    pps = (pages + p.splits - 1) / p.splits;
-    p.pages_per_split = (int)std::max<long long>(kStepWarps, (pps + kStepWarps - 1) / kStepWarps * kStepWarps);
+    p.min_units = 2 * kStepWarps;  // two pages for each warp: fewer, and the joining costs more than it gives
+    // as many CTAs as are resident at once (registers: 128 a thread for one tile of rows, 219 for two), or as there is work for
+    const long long items = (long long)b.seqs * kvh * ((rows + 8 * p.tiles - 1) / (8 * p.tiles));
+    const long long pages = std::max<long long>((b.max_ctx + kPage - 1) / kPage, 1);
+    const long long most = (long long)std::min((double)items * (pages + kItemUnits) / p.min_units + 1, 1e9);
+    p.grid = (int)std::min<long long>((p.tiles == 1 ? 4 : 2) * sms, most);
     return p;
 }
 
