@@ -822,7 +822,7 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     const long long most = (long long)b->max_rows * G;
     const bool prompt = c->head_dim != 32 && q->dtype != POX_F32 && most > kPromptRows;
     const bool step = !prompt || (b->seqs > 1 && b->rows != (unsigned long long)b->seqs * b->max_rows);
-    Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, G, ctx->num_sms,
+    Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, (int)c->head_dim, G, ctx->num_sms,
                                      prompt ? kPromptRows : 0x7fffffff);
     plan.device = ctx->device;
     rc = step ? kv8_scratch(ctx, st, c->head_dim, plan) : POX_OK;

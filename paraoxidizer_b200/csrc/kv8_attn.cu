@@ -11,16 +11,17 @@
 
 namespace pox {
 
-// Bytes of a page in the ring; pages in flight per warp (about 12 KB).
+// The ring of a warp: stages of two pages. Three CTAs to an SM at 128 dims, four below (registers and shared memory).
 template <int HD>
 struct StepRing {
-    static constexpr int kPageBytes = 32 * HD, kStages = HD == 128 ? 3 : HD == 64 ? 6 : 8;
+    static constexpr int kPageBytes = 32 * HD, kPairBytes = 2 * kPageBytes, kStages = HD == 128 ? 2 : 3;
 };
 
 // Two f16 from the low (high) two bytes of a word of int8.
 //   EXACT: the whole numbers q themselves.
-//   else:  (q + 128) 2^-24, the byte with its sign bit flipped as a subnormal f16: three instructions a word instead of
-//          five; the products' sums are then off by 128 2^-24 times the sum of the other operand, which the caller takes off.
+//   else:  (q + 128) 2^-24, the byte with its sign bit flipped as a subnormal f16: three instructions a word instead
+//          of five; the products' sums are then off by 128 2^-24 times the sum of the other operand, which the
+//          caller takes off.
 template <bool EXACT>
 __device__ __forceinline__ void bytes_to_f16(uint32_t v, uint32_t& r0, uint32_t& r1) {
     if constexpr (EXACT) {
@@ -36,38 +37,50 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {  // an 8 x 8 matrix
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+// D = A B + (c0, c1, c0, c1)
+__device__ __forceinline__ void mma_start(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1, float c0, float c1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t r;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a));
+    return r;
+}
 
-// The work of a launch is a line of units: for each sequence in turn, for each kv head and tile of 8 NT rows, kItemUnits
-// for starting on it and one for each page of the sequence. Every CTA takes an equal run of it, whatever the lengths are (with a CTA per split of the longest
-// context, a quarter of the SMs' time went by idle at three sequences of 131k, 116k and 61k tokens). An item that a run cuts leaves its part
-// in the CTA's place (0: of an item begun before, 1: of one that goes on), and the CTA that comes last joins them in order.
-// Within an item each warp streams whole pages (K and V of 16 tokens of the kv head, 32 HD contiguous bytes) through
-// a ring of its own with one bulk copy a page, and runs both
-// products transposed on mma.sync m16n8k16 with f32 accumulators, so that a page is the 16 rows of A and 8 query rows fill N:
+// The work of a launch is a line of units: for each sequence in turn, for each kv head and tile of 8 NT rows,
+// kItemUnits for starting on it and one for each page of the sequence. Every CTA takes an equal run of the line, whatever
+// the lengths are (with a CTA per split of the longest context, a quarter of the SMs' time went by idle at three sequences
+// of 131k, 109k and 61k tokens). A long item that a run's end cuts leaves its part in the CTA's place (0: of an item
+// begun before, 1: of one that goes on), and the CTA that comes last joins them in order.
+//
+// Within an item each warp streams whole pages (K and V of 16 tokens of the kv head, 32 HD contiguous bytes) through a ring of
+// its own with one bulk copy a page, two pages a turn, and runs both products transposed on mma.sync m16n8k16 with f32
+// accumulators, so that a page is the 16 rows of A and 8 query rows fill N:
 //   S^T (tokens x rows) = K Q^T,   O^T (dims x rows) = V^T P^T.
 // The MMA does not care in which order k and the rows of A run, so they run as the page's bytes lie: lane (g, t) takes
-// 16 dims of the tokens 4 (g / 2) + g % 2 (+ 2) for the first product and the four tokens 4 t .. 4 t + 3 of a dim for the
-// second, and P^T is S^T's own fragment, transposed in registers.
+// 16 dims of the tokens 4 (g / 2) + g % 2 (+ 2) for the first product and the four tokens 4 t .. 4 t + 3 of a dim for
+// the second, and P^T is S^T's own fragment, transposed in registers.
 // f32 rows: q and p as two f16 terms each (22 bits), bytes converted exactly. 16-bit rows: q exact, bytes with the
 // offset of bytes_to_f16; p two terms for f16 outputs of up to 8 rows (so that only the output's own rounding
 // remains), one for bf16 and for more rows (2^-11 of p).
 constexpr uint32_t kWholePages = 128;
 
-__device__ __forceinline__ unsigned long long div_u64(unsigned long long a, uint32_t b) {
-    return a >> 32 ? a / b : (uint32_t)a / b;  // (the long division is a hundred instructions)
-}
-
 template <int HD, typename T, int NT>
-__global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_step_kernel(Kv8Attn<T> a, Kv8StepPlan p) {
+__global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4) : 2)
+    kv8_attn_step_kernel(Kv8Attn<T> a, Kv8StepPlan p) {
     constexpr bool F32 = sizeof(T) == 4, PLO = F32 || (std::is_same<T, __half>::value && NT == 1);
-    constexpr int RT = 8 * NT, KW = HD / 16, NJ = HD / 16, PB = StepRing<HD>::kPageBytes, NST = StepRing<HD>::kStages;
+    constexpr int RT = 8 * NT, KW = HD / 16, NJ = HD / 16, NST = StepRing<HD>::kStages;
+    constexpr int PB = StepRing<HD>::kPageBytes, SB = StepRing<HD>::kPairBytes;
     constexpr float kOffset = 128.0f / 16777216.0f;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[kStepWarps][NST];
     __shared__ float ml[kStepWarps][2][RT];
     __shared__ uint32_t last_cta;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * NST * PB, bar = smem_u32(&bars[warp][0]);
+    const uint32_t ring = smem_u32(smem) + warp * NST * SB, bar = smem_u32(&bars[warp][0]);
     if (lane == 0) {
         for (int i = 0; i < NST; i++) mbar_init(bar + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -75,19 +88,25 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
     __syncwarp();
     // units of a sequence (one item at least, so that rows that see nothing are written), and where this CTA's run begins
     auto units = [&](uint32_t s, SeqSpan& q) -> unsigned long long {
-        if (!seq_span(a.b, s, q, a.err)) return 0;
+        if (s >= a.b.seqs || !seq_span(a.b, s, q, a.err)) return 0;
         const int rows = q.n * a.G;
         if (rows > p.most_rows) return 0;
-        return (unsigned long long)a.c.kvh * ((rows + RT - 1) / RT) * (kItemUnits + max((q.ctx + kPage - 1) / kPage, 1));
+        return (unsigned long long)(a.c.kvh * ((rows + RT - 1) / RT)) * (kItemUnits + max((q.ctx + kPage - 1) / kPage, 1));
     };
-    unsigned long long total = 0;
-    for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32) {
+    SeqSpan sq;
+    const unsigned long long mine = units(lane, sq);
+    unsigned long long all_units = mine;
+    for (uint32_t s0 = 32; s0 < a.b.seqs; s0 += 32) {
         SeqSpan q;
-        total += s0 + lane < a.b.seqs ? units(s0 + lane, q) : 0;
+        all_units += units(s0 + lane, q);
     }
 #pragma unroll
-    for (int k = 16; k; k >>= 1) total += __shfl_xor_sync(0xffffffffu, total, k);
-    const uint32_t run = max((uint32_t)div_u64(total + gridDim.x - 1, gridDim.x), (uint32_t)p.min_units);
+    for (int k = 16; k; k >>= 1) all_units += __shfl_xor_sync(0xffffffffu, all_units, k);
+    if (all_units >= 0xff000000u) {
+        if (tid == 0) atomicOr(a.err, kErrBatch);
+        return;
+    }
+    const uint32_t total = (uint32_t)all_units, run = max((total + gridDim.x - 1) / gridDim.x, (uint32_t)p.min_units);
     // An item of up to `whole` pages is not cut (joining costs about what 64 pages do), and none within `edge` of its
     // ends: the border goes to the nearer end.
     const uint32_t whole = min(kWholePages, 2 * run), edge = min(16u, run / 2);
@@ -95,16 +114,16 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
         if (all - kItemUnits <= whole) return 2 * u < all ? 0u : all;
         return u < kItemUnits + edge ? 0u : u > all - edge ? all : u;
     };
-    const unsigned long long x_begin = (unsigned long long)run * blockIdx.x, x_end = x_begin + run;
-    if (x_begin >= total) return;
-    uint32_t s = 0;
-    unsigned long long base = 0;  // the line's place where sequence s begins
+    if ((unsigned long long)run * blockIdx.x >= total) return;
+    const uint32_t x_begin = run * blockIdx.x, x_end = min(total - x_begin, run) + x_begin;
+    uint32_t s = 0, base = 0;  // the sequence that holds x_begin, and the line's place where it begins
     for (uint32_t s0 = 0;; s0 += 32) {
         SeqSpan q;
-        unsigned long long u = s0 + lane < a.b.seqs ? units(s0 + lane, q) : 0, sum = u;
+        const uint32_t u = s0 ? (uint32_t)units(s0 + lane, q) : (uint32_t)mine;
+        uint32_t sum = u;
 #pragma unroll
         for (int k = 1; k < 32; k *= 2) {
-            const unsigned long long y = __shfl_up_sync(0xffffffffu, sum, k);
+            const uint32_t y = __shfl_up_sync(0xffffffffu, sum, k);
             if (lane >= k) sum += y;
         }
         const unsigned m = __ballot_sync(0xffffffffu, base + sum > x_begin);
@@ -118,22 +137,20 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
 
     bool bad = false;
     int st = 0, ph = 0;
-    SeqSpan sq;
-    unsigned long long su = units(s, sq);
-    uint32_t all = kItemUnits + max((sq.ctx + kPage - 1) / kPage, 1);
-    uint32_t item = (uint32_t)div_u64(x_begin - base, all);
-    uint32_t u0 = border((uint32_t)(x_begin - base - (unsigned long long)item * all), all);  // of the item, this CTA's first unit
+    uint32_t su = (uint32_t)units(s, sq), all = kItemUnits + max((sq.ctx + kPage - 1) / kPage, 1);
+    uint32_t item = (x_begin - base) / all;
+    uint32_t u0 = border(x_begin - base - item * all, all);  // of the item, this CTA's first unit
     for (;; item++, u0 = 0) {  // the items of this CTA's run
-        unsigned long long x0 = base + (unsigned long long)item * all;  // where the item begins
-        while (x0 >= base + su) {  // the sequence is done
+        uint32_t x0 = base + item * all;  // where the item begins
+        while (x0 - base >= su) {  // the sequence is done
             base += su;
-            if (x0 >= total || base >= x_end) return;
-            su = units(++s, sq);
+            if (base >= x_end) return;
+            su = (uint32_t)units(++s, sq);
             all = kItemUnits + max((sq.ctx + kPage - 1) / kPage, 1);
             item = 0, x0 = base;
         }
         if (x0 >= x_end) return;
-        const uint32_t u1 = x0 + all <= x_end ? all : border((uint32_t)(x_end - x0), all);
+        const uint32_t u1 = all <= x_end - x0 ? all : border(x_end - x0, all);
         if (u0 >= u1) continue;
         const int rows = sq.n * a.G, tiles = (rows + RT - 1) / RT;
         // tiles of a sequence in the order first, last, second, ..: early ones see fewer pages of a chunk
@@ -144,8 +161,24 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
         // the CTA that holds the item's first part, and the parts: one more than the borders that cut it
         uint32_t c0 = blockIdx.x, ns = 1;
         if (u0 > 0 || u1 < all) {
-            const uint32_t i0 = (uint32_t)div_u64(x0 + kItemUnits + edge + run - 1, run), i1 = (uint32_t)div_u64(x0 + all - edge, run);
+            const uint32_t i0 = (x0 + kItemUnits + edge + run - 1) / run, i1 = (x0 + all - edge) / run;
             c0 = i0 - 1, ns = i1 - i0 + 2;
+        }
+
+        // the rows: lane (g, t) the dims of row g that t takes of a token (asked for before anything queues up behind
+        // the pages)
+        float qv[NT][KW][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int row = row0 + 8 * n + g;
+            const bool ok = row < rows;
+            const T* q = a.q.at((size_t)sq.r0 + (ok ? row / a.G : 0), h * a.G + (ok ? row % a.G : 0));
+#pragma unroll
+            for (int w = 0; w < KW; w++) {
+                const int d = HD == 32 ? 8 * t + 4 * w : 64 * (w / 4) + 16 * t + 4 * (w % 4);
+                if (ok) load4(q + d, a.vec, qv[n][w]);
+                else qv[n][w][0] = qv[n][w][1] = qv[n][w][2] = qv[n][w][3] = 0.f;
+            }
         }
 
         // this warp's pages: first, first + W, ..; lane i holds place and scales of the i-th of 32, and of the next 32
@@ -163,54 +196,48 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
                 there = blk >= 0 && (uint32_t)blk < a.c.num_blocks;
                 if (!there) atomicOr(a.err, kErrAttnPage);
                 e.place = there ? (size_t)blk * a.c.kvh + h : 0;
+                e.ab = *reinterpret_cast<const float2*>(a.c.scales + e.place * 2);
             }
             e.there = __ballot_sync(0xffffffffu, there);
             return e;
-        };
-        auto scales = [&](Entry& e, int i0) {
-            if (i0 + lane < cnt) e.ab = *reinterpret_cast<const float2*>(a.c.scales + e.place * 2);
         };
         // log2 b; a scale of 0 stands for zeros whatever the bytes: 1e-30 of them is nothing next to any other page
         float lb, ib;
         auto logs = [&](const Entry& e) {
             lb = log2f(fmaxf(e.ab.y, 1e-30f) + (e.ab.y - e.ab.y)), ib = 1.0f / fmaxf(e.ab.y, 1e-30f);
         };
-        auto fetch = [&](const Entry& e, int i, int st) {  // page i of this warp into its stage (one out of range: page 0, unread)
-            const size_t pl = __shfl_sync(0xffffffffu, (unsigned long long)e.place, i & 31);
+        // pages i and i + 1 of this warp into a stage (one out of range: page 0, unread)
+        auto fetch = [&](const Entry& e, int i, int st) {
+            const size_t p0 = __shfl_sync(0xffffffffu, (unsigned long long)e.place, i & 31),
+                         p1 = __shfl_sync(0xffffffffu, (unsigned long long)e.place, (i & 31) + 1);
             if (lane == 0) {
-                mbar_expect_tx(bar + 8 * st, PB);
-                bulk_g2s(ring + st * PB, a.c.pages + pl * PB, PB, bar + 8 * st);
+                const bool two = i + 1 < cnt;
+                mbar_expect_tx(bar + 8 * st, two ? SB : PB);
+                bulk_g2s(ring + st * SB, a.c.pages + p0 * PB, PB, bar + 8 * st);
+                if (two) bulk_g2s(ring + st * SB + PB, a.c.pages + p1 * PB, PB, bar + 8 * st);
             }
         };
         cur = entries(0);
-        for (int i = 0, k = st; i < min(cnt, NST); i++) {
+        for (int i = 0, k = st; i < min(cnt, 2 * NST); i += 2) {
             fetch(cur, i, k);
             if (++k == NST) k = 0;
         }
-        scales(cur, 0);
         logs(cur);
 
-        // B fragments of the rows: lane (g, t) the dims of row g that t takes of a token. Then, for the rows 2 t and 2 t + 1 that
-        // this lane's scores belong to: what takes a product to a score, its offset, and the last position seen
+        // B fragments of the rows. Then, for the rows 2 t and 2 t + 1 that this lane's scores belong to: what takes a
+        // product to a score, its offset, and the last position seen
         uint32_t qb[NT][F32 ? 2 : 1][KW][2];
         float qf[NT][2], qo[NT][2];
         int rpos[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const int row = row0 + 8 * n + g;
-            const bool ok = row < rows;
-            const T* q = a.q.at((size_t)sq.r0 + (ok ? row / a.G : 0), h * a.G + (ok ? row % a.G : 0));
-            float v[KW][4], m = 0.f;
-#pragma unroll
-            for (int w = 0; w < KW; w++) {
-                const int d = HD == 32 ? 8 * t + 4 * w : 64 * (w / 4) + 16 * t + 4 * (w % 4);
-                if (ok) load4(q + d, a.vec, v[w]);
-                else v[w][0] = v[w][1] = v[w][2] = v[w][3] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(v[w][i]));
-            }
             float f = 1.f, inv = 1.f, sum = 0.f;
             if constexpr (!std::is_same<T, __half>::value) {
+                float m = 0.f;
+#pragma unroll
+                for (int w = 0; w < KW; w++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(qv[n][w][i]));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 f = row_factor(m, inv);
@@ -219,7 +246,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
             for (int w = 0; w < KW; w++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const float x = v[w][2 * i] * f, y = v[w][2 * i + 1] * f;
+                    const float x = qv[n][w][2 * i] * f, y = qv[n][w][2 * i + 1] * f;
                     qb[n][0][w][i] = pack_f16(x, y);
                     if constexpr (F32) {
                         const float2 hi = unpack_f16(qb[n][0][w][i]);
@@ -239,76 +266,88 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
             }
         }
 
-        float o[NT][NJ][4], m[NT][2], l[NT][2], ps[NT][2];  // ps: the sum of p as the product sees it
+        // m: the reference (-inf until a row has seen something); ref: m, or 0; ps: the sum of p as the product sees
+        // it (a product with ones)
+        float o[NT][NJ][4], m[NT][2], ref[NT][2], l[NT][2], ps[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
             for (int j = 0; j < NJ; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; e++) m[n][e] = -INFINITY, l[n][e] = 0.f, ps[n][e] = 0.f;
+            for (int e = 0; e < 2; e++) m[n][e] = -INFINITY, ref[n][e] = 0.f, l[n][e] = 0.f, ps[n][e] = ps[n][2 + e] = 0.f;
         }
         const int tok = 4 * (g >> 1) + (g & 1);
-        for (int i = 0; i < cnt; i++) {
-            const int page = first + i * kStepWarps;
+        const uint32_t k_at = HD == 32 ? tok * HD + 8 * t : tok * HD + 16 * t, swap = HD == 128 ? (g & 1) << 6 : 0,
+                       v_at = kPage * HD + g * kPage + 4 * t;
+        for (int i = 0; i < cnt; i += 2) {
             if ((i & 31) == 0) {
                 if (i) cur = nxt, logs(cur);
                 nxt = entries(i + 32);
-                scales(nxt, i + 32);
             }
-            const uint32_t base = ring + st * PB;
+            const uint32_t at = ring + st * SB;
             bad = __any_sync(0xffffffffu, !mbar_wait(bar + 8 * st, ph));
-            const float pa = __shfl_sync(0xffffffffu, cur.ab.x, i & 31), pl = __shfl_sync(0xffffffffu, lb, i & 31),
-                        pi = __shfl_sync(0xffffffffu, ib, i & 31);
-            // S^T: tokens tok (rows g of A) and tok + 2 (rows g + 8); two chains of products
-            float sc[NT][2][4];
+            const int page = first + i * kStepWarps;
+            const bool open = (cur.there >> (i & 31) & 3) == 3 && (page + kStepWarps + 1) * kPage - 1 <= pmin;
+            float u[2][NT][4], pi[2];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int k = 0; k < 2; k++) {
+                const uint32_t kb = at + k * PB + k_at;
+                const float pa = __shfl_sync(0xffffffffu, cur.ab.x, (i & 31) + k),
+                            pl = __shfl_sync(0xffffffffu, lb, (i & 31) + k);
+                pi[k] = __shfl_sync(0xffffffffu, ib, (i & 31) + k);
+                // S^T: tokens tok (rows g of A) and tok + 2 (rows g + 8)
+                uint32_t kw[2][KW];
 #pragma unroll
-                for (int k = 0; k < 2; k++)
+                for (int r = 0; r < 2; r++) {
+                    if constexpr (HD == 32) {
+                        const uint2 x = lds64(kb + 2 * r * HD);
+                        kw[r][0] = x.x, kw[r][1] = x.y;
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) sc[n][k][e] = k == 0 ? qo[n][e & 1] : 0.f;
-            uint32_t kw[2][KW];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const uint32_t at = base + (tok + 2 * u) * HD;
-                if constexpr (HD == 32) {
-                    const uint2 x = lds64(at + 8 * t);
-                    kw[u][0] = x.x, kw[u][1] = x.y;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < HD / 64; c++) {
-                        const uint4 x = lds128(at + (HD == 128 ? (64 * c + 16 * t) ^ ((g & 1) << 6) : 16 * t));
-                        kw[u][4 * c] = x.x, kw[u][4 * c + 1] = x.y, kw[u][4 * c + 2] = x.z, kw[u][4 * c + 3] = x.w;
+                        for (int c = 0; c < HD / 64; c++) {
+                            const uint4 x = lds128(kb + 2 * r * HD + (c ? 64 - swap : swap));
+                            kw[r][4 * c] = x.x, kw[r][4 * c + 1] = x.y, kw[r][4 * c + 2] = x.z, kw[r][4 * c + 3] = x.w;
+                        }
                     }
                 }
+#pragma unroll
+                for (int w = 0; w < KW; w++) {
+                    uint32_t a0, a1, a2, a3;
+                    bytes_to_f16<F32>(kw[0][w], a0, a2);
+                    bytes_to_f16<F32>(kw[1][w], a1, a3);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        if (w == 0) mma_start(u[k][n], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1], qo[n][0], qo[n][1]);
+                        else mma_16816(u[k][n], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1]);
+                        if constexpr (F32) mma_16816(u[k][n], a0, a1, a2, a3, qb[n][F32][w][0], qb[n][F32][w][1]);
+                    }
+                }
+                // u of tokens tok, tok + 2 and rows 2 t, 2 t + 1
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) u[k][n][e] = fmaf(u[k][n][e], qf[n][e & 1] * pa, pl);
             }
+            if (!open) {
 #pragma unroll
-            for (int w = 0; w < KW; w++) {
-                uint32_t a0, a1, a2, a3;
-                bytes_to_f16<F32>(kw[0][w], a0, a2);
-                bytes_to_f16<F32>(kw[1][w], a1, a3);
+                for (int k = 0; k < 2; k++) {
+                    const bool seen = cur.there >> ((i & 31) + k) & 1;
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    mma_16816(sc[n][w & 1], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1]);
-                    if constexpr (F32) mma_16816(sc[n][w & 1], a0, a1, a2, a3, qb[n][F32][w][0], qb[n][F32][w][1]);
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (!seen || (page + k * kStepWarps) * kPage + tok + 2 * (e >> 1) > rpos[n][e & 1])
+                                u[k][n][e] = -INFINITY;
                 }
             }
-            // u of tokens tok, tok + 2 and rows 2 t, 2 t + 1
-            const bool seen = cur.there >> (i & 31) & 1, whole = page * kPage + kPage - 1 <= pmin && seen;
-            float u[NT][4];
             bool grow = false;
+            float mx[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const float f = qf[n][e] * pa;
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        float x = fmaf(sc[n][0][2 * k + e] + sc[n][1][2 * k + e], f, pl);
-                        if (!whole && (page * kPage + tok + 2 * k > rpos[n][e] || !seen)) x = -INFINITY;
-                        u[n][2 * k + e] = x;
-                    }
-                    grow |= fmaxf(u[n][e], u[n][2 + e]) > m[n][e] + 8.0f;
+                    mx[n][e] = fmaxf(fmaxf(u[0][n][e], u[0][n][2 + e]), fmaxf(u[1][n][e], u[1][n][2 + e]));
+                    grow |= mx[n][e] > m[n][e] + 8.0f;
                 }
             // the reference moves only when p would pass 2^8: after the first pages it hardly ever does
             if (__any_sync(0xffffffffu, grow)) {
@@ -316,66 +355,71 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float to = fmaxf(u[n][e], u[n][2 + e]);
+                        float to = mx[n][e];
 #pragma unroll
                         for (int k = 4; k < 32; k *= 2) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, k));
                         to = to > m[n][e] + 8.0f ? to : m[n][e];
                         const float f = m[n][e] == -INFINITY ? (to == -INFINITY ? 1.f : 0.f) : ex2(m[n][e] - to);
-                        m[n][e] = to;
-                        l[n][e] *= f, ps[n][e] *= f;
+                        m[n][e] = to, ref[n][e] = to == -INFINITY ? 0.f : to;
+                        l[n][e] *= f, ps[n][e] *= f, ps[n][2 + e] *= f;
 #pragma unroll
                         for (int j = 0; j < NJ; j++) o[n][j][e] *= f, o[n][j][2 + e] *= f;
                     }
             }
-            uint32_t pb[NT][PLO ? 2 : 1][2];  // B fragments of P^T: tokens 4 t, 4 t + 1 | 4 t + 2, 4 t + 3 of row g
+            uint32_t pb[2][NT][PLO ? 2 : 1][2];  // B fragments of P^T: tokens 4 t, 4 t + 1 | 4 t + 2, 4 t + 3 of row g
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float x[4], y[2] = {0.f, 0.f};
+            for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = ex2(u[n][e] - (m[n][e & 1] == -INFINITY ? 0.f : m[n][e & 1]));
+                for (int n = 0; n < NT; n++) {
+                    float x[4];
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const uint32_t hi = pack_f16(x[2 * k], x[2 * k + 1]);
-                    const float2 r = unpack_f16(hi);
-                    pb[n][0][k] = transpose8(hi);
-                    if constexpr (PLO) {
-                        const uint32_t lo = pack_f16(x[2 * k] - r.x, x[2 * k + 1] - r.y);
-                        pb[n][PLO][k] = transpose8(lo);
-                        y[0] += x[2 * k], y[1] += x[2 * k + 1];
-                    } else {
-                        y[0] += r.x, y[1] += r.y;
+                    for (int e = 0; e < 4; e++) x[e] = ex2(u[k][n][e] - ref[n][e & 1]);
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const uint32_t hi = pack_f16(x[2 * r], x[2 * r + 1]);
+                        pb[k][n][0][r] = transpose8(hi);
+                        if constexpr (PLO) {
+                            const float2 z = unpack_f16(hi);
+                            pb[k][n][PLO][r] = transpose8(pack_f16(x[2 * r] - z.x, x[2 * r + 1] - z.y));
+                        }
+                    }
+                    if constexpr (!F32) {
+                        constexpr uint32_t kOne = 0x3c003c00u;
+                        mma_16816(ps[n], kOne, kOne, kOne, kOne, pb[k][n][0][0], pb[k][n][0][1]);
+                        if constexpr (PLO) mma_16816(ps[n], kOne, kOne, kOne, kOne, pb[k][n][PLO][0], pb[k][n][PLO][1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        // (p in f32: a page's p may be nothing in f16 next to its part of l. An unseen page's scale may be anything.)
+                        const float y = x[e] + x[2 + e];
+                        if (open || y != 0.f) l[n][e] = fmaf(y, pi[k], l[n][e]);
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    if (y[e] != 0.f) l[n][e] = fmaf(y[e], pi, l[n][e]);  // (an unseen page's scale may be anything)
-                    if (!F32) ps[n][e] += y[e];
-                }
-            }
+            for (int j = 0; j < NJ; j++)
 #pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                uint32_t w0, w1, a0, a1, a2, a3;
-                const uint32_t at = base + kPage * HD + (16 * j + g) * kPage + 4 * t;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w0) : "r"(at));
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w1) : "r"(at + 8 * kPage));
-                bytes_to_f16<F32>(w0, a0, a2);
-                bytes_to_f16<F32>(w1, a1, a3);
+                for (int k = 0; k < 2; k++) {
+                    uint32_t a0, a1, a2, a3;
+                    const uint32_t vb = at + k * PB + v_at + 16 * j * kPage;
+                    bytes_to_f16<F32>(lds32(vb), a0, a2);
+                    bytes_to_f16<F32>(lds32(vb + 8 * kPage), a1, a3);
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    mma_16816(o[n][j], a0, a1, a2, a3, pb[n][0][0], pb[n][0][1]);
-                    if constexpr (PLO) mma_16816(o[n][j], a0, a1, a2, a3, pb[n][PLO][0], pb[n][PLO][1]);
+                    for (int n = 0; n < NT; n++) {
+                        mma_16816(o[n][j], a0, a1, a2, a3, pb[k][n][0][0], pb[k][n][0][1]);
+                        if constexpr (PLO) mma_16816(o[n][j], a0, a1, a2, a3, pb[k][n][PLO][0], pb[k][n][PLO][1]);
+                    }
                 }
-            }
             __syncwarp();  // every lane has read the stage
             if (bad) {  // a copy did not come in time: give the ones in flight as long again, and leave
-                for (int k = i; k < min(cnt, i + NST); k++) {
+                for (int k = i; k < min(cnt, i + 2 * NST); k += 2) {
                     mbar_wait(bar + 8 * st, ph);
                     if (++st == NST) st = 0, ph ^= 1;
                 }
                 if (lane == 0) atomicOr(a.err, kErrWaitRing);
                 break;
             }
-            if (i + NST < cnt) fetch(((i + NST) ^ i) & ~31 ? nxt : cur, i + NST, st);
+            const int to = i + 2 * NST;
+            if (to < cnt) fetch((to ^ i) & ~31 ? nxt : cur, to, st);
             if (++st == NST) st = 0, ph ^= 1;
         }
 
@@ -386,14 +430,11 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                float y = l[n][e], z = ps[n][e];
+                float y = l[n][e];
 #pragma unroll
-                for (int k = 4; k < 32; k *= 2) {
-                    y += __shfl_xor_sync(0xffffffffu, y, k);
-                    if (!F32) z += __shfl_xor_sync(0xffffffffu, z, k);
-                }
+                for (int k = 4; k < 32; k *= 2) y += __shfl_xor_sync(0xffffffffu, y, k);
                 if (g == 0) ml[warp][0][8 * n + 2 * t + e] = m[n][e], ml[warp][1][8 * n + 2 * t + e] = y;
-                off[n][e] = -128.0f * z;
+                off[n][e] = -128.0f * ps[n][e];
             }
         __syncthreads();
         float* os = reinterpret_cast<float*>(smem);  // [warp][RT][OS]
@@ -478,7 +519,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? 4 : 2) kv8_attn_ste
 
 template <int HD, typename T>
 cudaError_t launch_kv8_step(const Kv8Attn<T>& a, const Kv8StepPlan& p, cudaStream_t st) {
-    constexpr int smem = kStepWarps * StepRing<HD>::kStages * StepRing<HD>::kPageBytes;
+    constexpr int smem = kStepWarps * StepRing<HD>::kStages * StepRing<HD>::kPairBytes;
     static_assert(smem >= kStepWarps * 16 * (HD + 4) * 4, "the ring holds the warps' parts");
     auto go = [&](auto* kernel, std::atomic<uint32_t>& done) {
         const cudaError_t e = kv8_smem_once(kernel, smem, p.device, done);

@@ -36,17 +36,17 @@ struct Kv8StepPlan {
     size_t part_bytes(uint32_t hd) const { return (size_t)grid * 2 * 8 * tiles * (hd + 2) * sizeof(float); }
 };
 
-inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int G, int sms, int most_rows) {
+inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int hd, int G, int sms, int most_rows) {
     Kv8StepPlan p;
     p.most_rows = most_rows;
     const long long rows = std::min((long long)b.max_rows * G, (long long)most_rows);
     p.tiles = rows <= 8 ? 1 : 2;
     p.min_units = 2 * kStepWarps;  // two pages for each warp: fewer, and the joining costs more than it gives
-    // as many CTAs as are resident at once (registers: 128 a thread for one tile of rows, 219 for two), or as there is work for
+    // as many CTAs as are resident at once, or as there is work for
     const long long items = (long long)b.seqs * kvh * ((rows + 8 * p.tiles - 1) / (8 * p.tiles));
     const long long pages = std::max<long long>((b.max_ctx + kPage - 1) / kPage, 1);
     const long long most = (long long)std::min((double)items * (pages + kItemUnits) / p.min_units + 1, 1e9);
-    p.grid = (int)std::min<long long>((p.tiles == 1 ? 4 : 2) * sms, most);
+    p.grid = (int)std::min<long long>((p.tiles == 1 ? (hd == 128 ? 3 : 4) : 2) * sms, most);
     return p;
 }
 
