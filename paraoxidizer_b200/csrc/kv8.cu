@@ -29,6 +29,8 @@ struct QkArgs {
 // Any shape: one warp per (row, head), a pass for the sum of squares and one for the pairs.
 template <typename T>
 __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(QkArgs<T> a) {
+    pdl_wait();
+    pdl_launch_dependents();
     const int nh = a.heads[0] + a.heads[1], lane = threadIdx.x & 31;
     const unsigned long long item = (unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (item >= (unsigned long long)a.rows * nh) return;
@@ -75,6 +77,8 @@ constexpr int kQkAhead = 4;
 template <typename T, int L, bool HALF>
 __global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(QkArgs<T> a, int steps, int groups) {
     constexpr int V = 16 / sizeof(T), HW = 32 / L, P = V / 2;
+    pdl_wait();
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31, c = lane % L, nh = a.heads[0] + a.heads[1], rot = a.rope.rot;
     const unsigned long long item = (unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const uint32_t r = (uint32_t)(item / groups);
@@ -289,6 +293,8 @@ enum { kTurnAny = 0, kTurnNone = 1, kTurnHalf = 2, kTurnPairs = 3 };
 template <int HD, typename T, int TURN>
 __global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uint32_t items) {
     constexpr int L = HD / 4, UC = 128 / (2 * L), NT = kPage / 2;
+    pdl_wait();
+    pdl_launch_dependents();
     __shared__ float red[4];
     const int lane = threadIdx.x & 31, c = threadIdx.x % L, hi = threadIdx.x / L & 1, t0 = NT * hi;
     const unsigned long long u = (unsigned long long)blockIdx.x * UC + threadIdx.x / (2 * L);
@@ -477,6 +483,8 @@ template <int HD, typename T>
 __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8Cache cache, Kv8Batch b, RowsView<T> k, RowsView<T> v,
                                                        uint32_t items, int vec, int* err) {
     constexpr int L = HD / 4, UW = 32 / L;
+    pdl_wait();
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31, c = lane % L;
     const unsigned long long u = ((unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * UW + lane / L;
     const uint32_t item = min((uint32_t)(u / (2 * cache.kvh)), items - 1);
@@ -648,8 +656,7 @@ static cudaError_t launch_qk(pox_cuda_ctx* ctx, const pox_qk_norm_rope* a, cudaS
                   ((k.in[i].row | k.in[i].head | k.out[i].row | k.out[i].head) % V) == 0;
     if (!vec) {
         const unsigned long long items = (unsigned long long)a->rows * nh;
-        qk_norm_rope_any_kernel<T><<<(unsigned)((items + 7) / 8), 256, 0, st>>>(k);
-        return cudaGetLastError();
+        return launch_pdl(qk_norm_rope_any_kernel<T>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, st, k);
     }
     // as many groups of heads to a warp as leave every SM its 32 warps
     const int all = (nh * L + 31) / 32;
@@ -657,19 +664,14 @@ static cudaError_t launch_qk(pox_cuda_ctx* ctx, const pox_qk_norm_rope* a, cudaS
                                                std::min(all, 10));
     const int groups = (all + steps - 1) / steps;
     const unsigned grid = (unsigned)(((unsigned long long)a->rows * groups + 7) / 8);
-    auto go = [&](auto half) {
+    auto go = [&](auto* kernel) { return launch_pdl(kernel, dim3(grid), dim3(256), 0, st, k, steps, groups); };
+    auto by_lanes = [&](auto half) {
         constexpr bool H = decltype(half)::value;
-        switch (L) {
-            case 2: qk_norm_rope_kernel<T, 2, H><<<grid, 256, 0, st>>>(k, steps, groups); break;
-            case 4: qk_norm_rope_kernel<T, 4, H><<<grid, 256, 0, st>>>(k, steps, groups); break;
-            case 8: qk_norm_rope_kernel<T, 8, H><<<grid, 256, 0, st>>>(k, steps, groups); break;
-            case 16: qk_norm_rope_kernel<T, 16, H><<<grid, 256, 0, st>>>(k, steps, groups); break;
-            default: qk_norm_rope_kernel<T, 32, H><<<grid, 256, 0, st>>>(k, steps, groups);
-        }
+        return L == 2 ? go(qk_norm_rope_kernel<T, 2, H>) : L == 4 ? go(qk_norm_rope_kernel<T, 4, H>)
+             : L == 8 ? go(qk_norm_rope_kernel<T, 8, H>) : L == 16 ? go(qk_norm_rope_kernel<T, 16, H>)
+                                                                    : go(qk_norm_rope_kernel<T, 32, H>);
     };
-    if (k.rope.half) go(std::true_type());
-    else go(std::false_type());
-    return cudaGetLastError();
+    return k.rope.half ? by_lanes(std::true_type()) : by_lanes(std::false_type());
 }
 
 static uint32_t page_items(const pox_kv8_batch* b) {
@@ -690,11 +692,11 @@ static cudaError_t launch_append(pox_cuda_ctx* ctx, const pox_kv8_cache* c, cons
     const unsigned grid = (unsigned)((lanes + 127) / 128);
     const RopeView& r = a.rope;
     const bool vec = vec4(k) && vec4(v) && ((uintptr_t)r.table & 15) == 0;
-    if (vec && !r.rot) kv8_append_kernel<HD, T, kTurnNone><<<grid, 128, 0, st>>>(a, items);
-    else if (vec && r.half && r.rot % 8 == 0) kv8_append_kernel<HD, T, kTurnHalf><<<grid, 128, 0, st>>>(a, items);
-    else if (vec && !r.half && r.rot % 4 == 0) kv8_append_kernel<HD, T, kTurnPairs><<<grid, 128, 0, st>>>(a, items);
-    else kv8_append_kernel<HD, T, kTurnAny><<<grid, 128, 0, st>>>(a, items);
-    return cudaGetLastError();
+    auto go = [&](auto* kernel) { return launch_pdl(kernel, dim3(grid), dim3(128), 0, st, a, items); };
+    return vec && !r.rot                      ? go(kv8_append_kernel<HD, T, kTurnNone>)
+           : vec && r.half && r.rot % 8 == 0  ? go(kv8_append_kernel<HD, T, kTurnHalf>)
+           : vec && !r.half && r.rot % 4 == 0 ? go(kv8_append_kernel<HD, T, kTurnPairs>)
+                                              : go(kv8_append_kernel<HD, T, kTurnAny>);
 }
 
 template <int HD, typename T>
@@ -702,9 +704,8 @@ static cudaError_t launch_read(pox_cuda_ctx* ctx, const pox_kv8_cache* c, const 
                                const pox_rows* v, cudaStream_t st) {
     const uint32_t items = page_items(b);
     const unsigned long long lanes = (unsigned long long)items * c->kv_heads * 2 * (HD / 4);
-    kv8_read_kernel<HD, T><<<(unsigned)((lanes + 127) / 128), 128, 0, st>>>(
-        cache_view(c), batch_view(b), rows_view<T>(*k), rows_view<T>(*v), items, vec4(k) && vec4(v), ctx->err_dev);
-    return cudaGetLastError();
+    return launch_pdl(kv8_read_kernel<HD, T>, dim3((unsigned)((lanes + 127) / 128)), dim3(128), 0, st, cache_view(c),
+                      batch_view(b), rows_view<T>(*k), rows_view<T>(*v), items, vec4(k) && vec4(v), ctx->err_dev);
 }
 
 // f.template operator()<HD, T>() for the head dim and the rows' type

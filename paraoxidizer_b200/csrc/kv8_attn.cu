@@ -82,10 +82,12 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t ring = smem_u32(smem) + warp * NST * SB, bar = smem_u32(&bars[warp][0]);
     if (lane == 0) {
-        for (int i = 0; i < NST; i++) mbar_init(bar + 8 * i, 1);
+        for (int i = 0; i < NST; i++) mbar_init(bar + 8 * i, 2);  // the lanes of its two pages
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
+    pdl_wait();
+    pdl_launch_dependents();
     // units of a sequence (one item at least, so that rows that see nothing are written), and where this CTA's run begins
     auto units = [&](uint32_t s, SeqSpan& q) -> unsigned long long {
         if (s >= a.b.seqs || !seq_span(a.b, s, q, a.err)) return 0;
@@ -181,22 +183,23 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
             }
         }
 
-        // this warp's pages: first, first + W, ..; lane i holds place and scales of the i-th of 32, and of the next 32
+        // this warp's pages: first, first + W, ..; lane i looks after the i-th of 32, and of the next 32: their
+        // entries are asked for 32 pages ahead, their scales when the entries are there
         const int first = page0 + warp, cnt = first < page1 && !bad ? (page1 - first + kStepWarps - 1) / kStepWarps : 0;
         struct Entry {
-            size_t place;
+            const int8_t* page;  // (one out of range: page 0, unread)
             float2 ab;
             unsigned there;
         } cur, nxt;
-        auto entries = [&](int i0) {
-            Entry e{0, make_float2(0.f, 0.f), 0};
-            bool there = false;
-            if (i0 + lane < cnt) {
-                const int blk = a.b.btab[(size_t)s * a.b.mbps + first + (i0 + lane) * kStepWarps];
-                there = blk >= 0 && (uint32_t)blk < a.c.num_blocks;
+        auto entry = [&](int i) { return i < cnt ? a.b.btab[(size_t)s * a.b.mbps + first + i * kStepWarps] : 0; };
+        auto resolve = [&](int blk, int i) {
+            Entry e{nullptr, make_float2(0.f, 0.f), 0};
+            const bool there = i < cnt && blk >= 0 && (uint32_t)blk < a.c.num_blocks;
+            if (i < cnt) {
                 if (!there) atomicOr(a.err, kErrAttnPage);
-                e.place = there ? (size_t)blk * a.c.kvh + h : 0;
-                e.ab = *reinterpret_cast<const float2*>(a.c.scales + e.place * 2);
+                const size_t place = there ? (size_t)blk * a.c.kvh + h : 0;
+                e.page = a.c.pages + place * PB;
+                e.ab = *reinterpret_cast<const float2*>(a.c.scales + place * 2);
             }
             e.there = __ballot_sync(0xffffffffu, there);
             return e;
@@ -206,22 +209,24 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
         auto logs = [&](const Entry& e) {
             lb = log2f(fmaxf(e.ab.y, 1e-30f) + (e.ab.y - e.ab.y)), ib = 1.0f / fmaxf(e.ab.y, 1e-30f);
         };
-        // pages i and i + 1 of this warp into a stage (one out of range: page 0, unread)
-        auto fetch = [&](const Entry& e, int i, int st) {
-            const size_t p0 = __shfl_sync(0xffffffffu, (unsigned long long)e.place, i & 31),
-                         p1 = __shfl_sync(0xffffffffu, (unsigned long long)e.place, (i & 31) + 1);
-            if (lane == 0) {
-                const bool two = i + 1 < cnt;
-                mbar_expect_tx(bar + 8 * st, two ? SB : PB);
-                bulk_g2s(ring + st * SB, a.c.pages + p0 * PB, PB, bar + 8 * st);
-                if (two) bulk_g2s(ring + st * SB + PB, a.c.pages + p1 * PB, PB, bar + 8 * st);
+        // pages i and i + 1 of this warp into a stage, by the lanes that look after them
+        auto fetch = [&](const int8_t* page, int i, int st) {
+            const uint32_t k = lane - (i & 31);
+            if (k < 2) {
+                if (i + (int)k < cnt) {
+                    mbar_expect_tx(bar + 8 * st, PB);
+                    bulk_g2s(ring + st * SB + k * PB, page, PB, bar + 8 * st);
+                } else {
+                    mbar_arrive(bar + 8 * st);
+                }
             }
         };
-        cur = entries(0);
+        cur = resolve(entry(lane), lane);
         for (int i = 0, k = st; i < min(cnt, 2 * NST); i += 2) {
-            fetch(cur, i, k);
+            fetch(cur.page, i, k);
             if (++k == NST) k = 0;
         }
+        int ahead = entry(32 + lane);
         logs(cur);
 
         // B fragments of the rows. Then, for the rows 2 t and 2 t + 1 that this lane's scores belong to: what takes a
@@ -280,9 +285,10 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
         const uint32_t k_at = HD == 32 ? tok * HD + 8 * t : tok * HD + 16 * t, swap = HD == 128 ? (g & 1) << 6 : 0,
                        v_at = kPage * HD + g * kPage + 4 * t;
         for (int i = 0; i < cnt; i += 2) {
-            if ((i & 31) == 0) {
-                if (i) cur = nxt, logs(cur);
-                nxt = entries(i + 32);
+            if ((i & 31) == 8) nxt = resolve(ahead, (i & ~31) + 32 + lane);
+            if ((i & 31) == 0 && i) {
+                cur = nxt, logs(cur);
+                ahead = entry(i + 32 + lane);
             }
             const uint32_t at = ring + st * SB;
             bad = __any_sync(0xffffffffu, !mbar_wait(bar + 8 * st, ph));
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                 break;
             }
             const int to = i + 2 * NST;
-            if (to < cnt) fetch((to ^ i) & ~31 ? nxt : cur, to, st);
+            if (to < cnt) fetch((to ^ i) & ~31 ? nxt.page : cur.page, to, st);
             if (++st == NST) st = 0, ph ^= 1;
         }
 
@@ -524,8 +530,7 @@ cudaError_t launch_kv8_step(const Kv8Attn<T>& a, const Kv8StepPlan& p, cudaStrea
     auto go = [&](auto* kernel, std::atomic<uint32_t>& done) {
         const cudaError_t e = kv8_smem_once(kernel, smem, p.device, done);
         if (e != cudaSuccess) return e;
-        kernel<<<p.grid, 32 * kStepWarps, smem, st>>>(a, p);
-        return cudaGetLastError();
+        return launch_pdl(kernel, dim3(p.grid), dim3(32 * kStepWarps), smem, st, a, p);
     };
     static std::atomic<uint32_t> done1{0}, done2{0};
     return p.tiles == 1 ? go(&kv8_attn_step_kernel<HD, T, 1>, done1) : go(&kv8_attn_step_kernel<HD, T, 2>, done2);

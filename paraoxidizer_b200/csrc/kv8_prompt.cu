@@ -65,6 +65,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
     const uint32_t full = smem_u32(bars), empty = full + 8 * NST, sfull = empty + 8 * NST, pready = sfull + 16,
                    ofull = pready + 16;
 
+    pdl_wait();
+    pdl_launch_dependents();
     // long tiles first: the last rows of a sequence see the most tokens
     const uint32_t pairs = a.b.seqs * (uint32_t)a.c.kvh, tiles = gridDim.x / pairs;
     const uint32_t h = blockIdx.x % a.c.kvh, s = blockIdx.x / a.c.kvh % a.b.seqs;
@@ -365,8 +367,8 @@ cudaError_t launch_kv8_prompt(const Kv8Attn<T>& a, int min_rows, int device, cud
     const cudaError_t e = kv8_smem_once(&kv8_attn_prompt_kernel<HD, T>, smem, device, done);
     if (e != cudaSuccess) return e;
     const unsigned long long tiles = ((unsigned long long)a.b.max_rows * a.G + 255) / 256;
-    kv8_attn_prompt_kernel<HD, T><<<(unsigned)(tiles * a.b.seqs * a.c.kvh), kPromptThreads, smem, st>>>(a, min_rows);
-    return cudaGetLastError();
+    return launch_pdl(kv8_attn_prompt_kernel<HD, T>, dim3((unsigned)(tiles * a.b.seqs * a.c.kvh)), dim3(kPromptThreads), smem,
+                      st, a, min_rows);
 }
 
 #define POX_KV8_PROMPT(HD)                                                                                  \
