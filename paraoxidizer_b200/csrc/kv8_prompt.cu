@@ -24,15 +24,39 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]), "r"(taddr)
-        : "memory");
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
+}
+// 32 columns of the warp's lanes, on their way; tmem_here(v) for each of them after tmem_wait_ld().
+__device__ __forceinline__ void tmem_ask32(uint32_t taddr, float* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_here(float* v) {  // (no instruction: uses of v stay behind the wait)
+    asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
+}
+template <int N>
+__device__ __forceinline__ void regs_more() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_less() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 constexpr int kPromptKeys = 128;                   // tokens of a tile: 8 pages
-constexpr int kPromptThreads = 32 * (4 + 4 + 4 + 1);  // two softmax warpgroups, the converters, the MMA warp
+constexpr int kPromptThreads = 512;  // two softmax warpgroups, the converters, the MMA warp's group
+// registers of a thread of each group; the launch gives 128 to all, and these sum to as much
+constexpr int kSoftmaxRegs = 192, kConvertRegs = 96, kMmaRegs = 32;
+static_assert(2 * kSoftmaxRegs + kConvertRegs + kMmaRegs <= 4 * 128, "more registers than the launch has");
 
 template <int HD>
 struct PromptSmem {
@@ -130,6 +154,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
     bool bad = false;
 
     if (warp < 8) {  // ---- softmax of tile ti
+        regs_more<kSoftmaxRegs>();
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tm + TS + 128 * ti + lanes,
                        to = tm + TO + HD * ti + lanes;
         const int rpos = mine ? pos0 + row / a.G : 0x3fffffff;
@@ -158,23 +183,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
                 if (bad) break;
                 tc_fence_after();
                 const bool cut = j * kPromptKeys + kPromptKeys - 1 > wpos;
+                // the tile's row in registers: the maximum of u a page at a time (its scales are one factor, one term)
+                float x[kPromptKeys];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_ask32(ts + 32 * c, x + 32 * c);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_here(x + 32 * c);
                 float mx = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float x[32];
-                    tmem_ld32(ts + 32 * c, x);
+                for (int g = 0; g < 8; g++) {
+                    const float f = qf * __shfl_sync(0xffffffffu, ka, g), pl = __shfl_sync(0xffffffffu, lb, g);
+                    if (cut) {
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const float f = qf * __shfl_sync(0xffffffffu, ka, 2 * c + g),
-                                    pl = __shfl_sync(0xffffffffu, lb, 2 * c + g);
-                        float y = -INFINITY;
+                        for (int i = 0; i < 16; i++)
+                            mx = fmaxf(mx, j * kPromptKeys + 16 * g + i > rpos ? -INFINITY : fmaf(x[16 * g + i], f, pl));
+                    } else {
+                        float y[2] = {x[16 * g], x[16 * g + 1]};
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            float z = x[16 * g + i];
-                            if (cut && j * kPromptKeys + 32 * c + 16 * g + i > rpos) z = -INFINITY;
-                            y = fmaxf(y, z);
-                        }
-                        mx = fmaxf(mx, fmaf(y, f, pl));
+                        for (int i = 2; i < 16; i += 2) y[0] = fmaxf(y[0], x[16 * g + i]), y[1] = fmaxf(y[1], x[16 * g + i + 1]);
+                        mx = fmaxf(mx, fmaf(fmaxf(y[0], y[1]), f, pl));
                     }
                 }
                 if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
@@ -184,39 +212,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
                     l *= f;
                     if (j) {
 #pragma unroll
-                        for (int c = 0; c < HD / 32; c++) {
-                            float x[32];
-                            tmem_ld32(to + 32 * c, x);
+                        for (int c = 0; c < HD / 16; c++) {
+                            float y[16];
+                            tmem_ld16(to + 16 * c, y);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) x[i] *= f;
-                            tmem_st32(to + 32 * c, x);
+                            for (int i = 0; i < 16; i++) y[i] *= f;
+                            tmem_st16(to + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(y));
                         }
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    float x[32];
-                    tmem_ld32(ts + 32 * c, x);
                     uint32_t hi[16];
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const float f = qf * __shfl_sync(0xffffffffu, ka, 2 * c + g),
-                                    pl = __shfl_sync(0xffffffffu, lb, 2 * c + g) - ref,
-                                    pi = __shfl_sync(0xffffffffu, ib, 2 * c + g);
-                        float sum = 0.f;
+                    for (int g = 2 * c; g < 2 * c + 2; g++) {
+                        const float f = qf * __shfl_sync(0xffffffffu, ka, g), pl = __shfl_sync(0xffffffffu, lb, g) - ref,
+                                    pi = __shfl_sync(0xffffffffu, ib, g);
+                        const uint64_t f2 = pair2(f, f), pl2 = pair2(pl, pl);
+                        uint64_t sum2 = 0;
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            float z = fmaf(x[16 * g + i], f, pl);
-                            if (cut && j * kPromptKeys + 32 * c + 16 * g + i > rpos) z = -INFINITY;
-                            x[16 * g + i] = ex2(z);
-                            sum += x[16 * g + i];
+                        for (int i = 0; i < 16; i += 2) {
+                            float2 z = both(fma2(pair2(x[16 * g + i], x[16 * g + i + 1]), f2, pl2));
+                            if (cut) {
+                                if (j * kPromptKeys + 16 * g + i > rpos) z.x = -INFINITY;
+                                if (j * kPromptKeys + 16 * g + i + 1 > rpos) z.y = -INFINITY;
+                            }
+                            z.x = ex2(z.x), z.y = ex2(z.y);
+                            sum2 = add2(sum2, pair2(z.x, z.y));
+                            hi[8 * (g & 1) + i / 2] = pack_f16(z.x, z.y);
                         }
-                        if (sum != 0.f) l = fmaf(sum, pi, l);
+                        const float sum = both(sum2).x + both(sum2).y;
+                        if (sum != 0.f) l = fmaf(sum, pi, l);  // (an unseen page's scale may be anything)
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; i++) hi[i] = pack_f16(x[2 * i], x[2 * i + 1]);
-                    tmem_st16(ts + 16 * c, hi);  // over columns of S that have been read
+                    tmem_st16(ts + 16 * c, hi);  // over columns of S
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -242,6 +271,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
             }
         }
     } else if (warp < 12) {  // ---- converters: pages 2 w and 2 w + 1 of each tile
+        regs_less<kConvertRegs>();
         const int w = warp - 8, b = lane & 7, g = lane >> 3;
         constexpr int NI = HD / 16;  // 16-byte pieces of K (or V) per lane and tile
         uint4 kr[NI], vr[NI];
@@ -306,7 +336,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
             }
             ready(st);
         }
-    } else if (lane == 0 && nk) {  // ---- the products
+    } else {  // ---- the products: one thread of warp 12
+        regs_less<kMmaRegs>();
+        if (warp == 12 && lane == 0 && nk) {
         constexpr uint32_t is = umma_idesc_f16(128, kPromptKeys), ip = umma_idesc_f16(128, HD);
         auto wait_full = [&](int n) {
             if (!bad) bad = !mbar_wait(full + 8 * (n % NST), (n / NST) & 1);
@@ -349,6 +381,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
         }
         umma_commit(ofull);
         if (bad) mbar_wait(ofull, 0);  // what was issued ends before the tensor memory is given back
+        }
     }
     if (bad && lane == 0) atomicOr(a.err, kErrWaitRing);
     tc_fence_before();
