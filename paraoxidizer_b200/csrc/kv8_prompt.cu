@@ -42,6 +42,11 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_here(float* v) {  // (no instruction: uses of v stay behind the wait)
     asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 template <int N>
 __device__ __forceinline__ void regs_more() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -159,7 +164,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
                        to = tm + TO + HD * ti + lanes;
         const int rpos = mine ? pos0 + row / a.G : 0x3fffffff;
         const int wpos = pos0 + (row0 + 32 * warp) / a.G;  // the first row of the warp sees no further
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, ref = 0.f, l = 0.f;
         if (ti < nt) {
             // lane i < 8 looks after page i of a tile: its entry two tiles ahead, its scales one tile ahead
             auto entry = [&](int j) {
@@ -182,71 +187,76 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
                 if (!bad) bad = __any_sync(0xffffffffu, !mbar_wait(sfull + 8 * ti, j & 1));
                 if (bad) break;
                 tc_fence_after();
-                const bool cut = j * kPromptKeys + kPromptKeys - 1 > wpos;
-                // the tile's row in registers: the maximum of u a page at a time (its scales are one factor, one term)
+                // the tile's row in registers
                 float x[kPromptKeys];
 #pragma unroll
                 for (int c = 0; c < 4; c++) tmem_ask32(ts + 32 * c, x + 32 * c);
+                float f[8], pl[8];  // u = S f + pl within a page
+#pragma unroll
+                for (int g = 0; g < 8; g++)
+                    f[g] = qf * __shfl_sync(0xffffffffu, ka, g), pl[g] = __shfl_sync(0xffffffffu, lb, g);
                 tmem_wait_ld();
 #pragma unroll
                 for (int c = 0; c < 4; c++) tmem_here(x + 32 * c);
-                float mx = -INFINITY;
+                const int left = rpos - j * kPromptKeys;  // the last of the tile's tokens that the row sees
+                auto softmax = [&](auto masked) {
+                    constexpr bool CUT = decltype(masked)::value;
+                    float mx = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < 8; g++) {
-                    const float f = qf * __shfl_sync(0xffffffffu, ka, g), pl = __shfl_sync(0xffffffffu, lb, g);
-                    if (cut) {
+                    for (int g = 0; g < 8; g++) {
+                        const float* y = x + 16 * g;
+                        if (CUT) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            mx = fmaxf(mx, j * kPromptKeys + 16 * g + i > rpos ? -INFINITY : fmaf(x[16 * g + i], f, pl));
-                    } else {
-                        float y[2] = {x[16 * g], x[16 * g + 1]};
-#pragma unroll
-                        for (int i = 2; i < 16; i += 2) y[0] = fmaxf(y[0], x[16 * g + i]), y[1] = fmaxf(y[1], x[16 * g + i + 1]);
-                        mx = fmaxf(mx, fmaf(fmaxf(y[0], y[1]), f, pl));
-                    }
-                }
-                if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
-                    const float go = mx > m + 8.0f ? mx : m;
-                    const float f = m == -INFINITY ? (go == -INFINITY ? 1.f : 0.f) : ex2(m - go);
-                    m = go;
-                    l *= f;
-                    if (j) {
-#pragma unroll
-                        for (int c = 0; c < HD / 16; c++) {
-                            float y[16];
-                            tmem_ld16(to + 16 * c, y);
-#pragma unroll
-                            for (int i = 0; i < 16; i++) y[i] *= f;
-                            tmem_st16(to + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(y));
+                            for (int i = 0; i < 16; i++) mx = fmaxf(mx, 16 * g + i > left ? -INFINITY : fmaf(y[i], f[g], pl[g]));
+                        } else {
+                            const float y0 = max3(y[0], y[1], y[2]), y1 = max3(y[3], y[4], y[5]), y2 = max3(y[6], y[7], y[8]),
+                                        y3 = max3(y[9], y[10], y[11]), y4 = max3(y[12], y[13], y[14]);
+                            mx = fmaxf(mx, fmaf(max3(max3(y0, y1, y2), max3(y3, y4, y[15]), y0), f[g], pl[g]));
                         }
                     }
-                }
-                const float ref = m == -INFINITY ? 0.f : m;
+                    if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
+                        const float go = mx > m + 8.0f ? mx : m;
+                        const float d = m == -INFINITY ? (go == -INFINITY ? 1.f : 0.f) : ex2(m - go);
+                        m = go, ref = go == -INFINITY ? 0.f : go;
+                        l *= d;
+                        if (j) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t hi[16];
+                            for (int c = 0; c < HD / 16; c++) {
+                                float y[16];
+                                tmem_ld16(to + 16 * c, y);
 #pragma unroll
-                    for (int g = 2 * c; g < 2 * c + 2; g++) {
-                        const float f = qf * __shfl_sync(0xffffffffu, ka, g), pl = __shfl_sync(0xffffffffu, lb, g) - ref,
-                                    pi = __shfl_sync(0xffffffffu, ib, g);
-                        const uint64_t f2 = pair2(f, f), pl2 = pair2(pl, pl);
-                        uint64_t sum2 = 0;
-#pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            float2 z = both(fma2(pair2(x[16 * g + i], x[16 * g + i + 1]), f2, pl2));
-                            if (cut) {
-                                if (j * kPromptKeys + 16 * g + i > rpos) z.x = -INFINITY;
-                                if (j * kPromptKeys + 16 * g + i + 1 > rpos) z.y = -INFINITY;
+                                for (int i = 0; i < 16; i++) y[i] *= d;
+                                tmem_st16(to + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(y));
                             }
-                            z.x = ex2(z.x), z.y = ex2(z.y);
-                            sum2 = add2(sum2, pair2(z.x, z.y));
-                            hi[8 * (g & 1) + i / 2] = pack_f16(z.x, z.y);
                         }
-                        const float sum = both(sum2).x + both(sum2).y;
-                        if (sum != 0.f) l = fmaf(sum, pi, l);  // (an unseen page's scale may be anything)
                     }
-                    tmem_st16(ts + 16 * c, hi);  // over columns of S
-                }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t hi[16];
+#pragma unroll
+                        for (int g = 2 * c; g < 2 * c + 2; g++) {
+                            const float off = pl[g] - ref, pi = __shfl_sync(0xffffffffu, ib, g);
+                            const uint64_t f2 = pair2(f[g], f[g]), off2 = pair2(off, off);
+                            uint64_t sum2 = 0;
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                float2 z = both(fma2(pair2(x[16 * g + i], x[16 * g + i + 1]), f2, off2));
+                                if (CUT) {
+                                    if (16 * g + i > left) z.x = -INFINITY;
+                                    if (16 * g + i + 1 > left) z.y = -INFINITY;
+                                }
+                                z.x = ex2(z.x), z.y = ex2(z.y);
+                                sum2 = add2(sum2, pair2(z.x, z.y));
+                                hi[8 * (g & 1) + i / 2] = pack_f16(z.x, z.y);
+                            }
+                            const float sum = both(sum2).x + both(sum2).y;
+                            if (!CUT || sum != 0.f) l = fmaf(sum, pi, l);  // (an unseen page's scale may be anything)
+                        }
+                        tmem_st16(ts + 16 * c, hi);  // over columns of S
+                    }
+                };
+                if (j * kPromptKeys + kPromptKeys - 1 > wpos) softmax(std::true_type());
+                else softmax(std::false_type());
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
