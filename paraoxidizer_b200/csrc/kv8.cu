@@ -605,6 +605,18 @@ static Kv8Batch batch_view(const pox_kv8_batch* b) {
 
 constexpr int kPromptRows = 64;
 
+// Which of the attention's kernels a batch of more rows should take, from the bounds that the host knows. The step kernel
+// spreads rows by 16 and the context over the whole GPU, a page of a tile at about 0.65 ns (head dim 128; 64: 0.46); a CTA of
+// the prompt kernel walks the context for 256 rows, 128 tokens in 3.0 us (up to 128 rows 2.4; head dim 64: 2.5,
+// 2.05). Measured both ways: one sequence of 128 tokens x 4 heads at 4096 tokens, 8 kv heads of 128: 57 us against 98;
+// eight of them: 350 against 105; eight of 32 tokens: 101 against 82; at 32768 tokens one of 256: 578 against 625.
+static bool prompt_is_faster(const pox_kv8_cache* c, const pox_kv8_batch* b, int G, int sms) {
+    const double rows = (double)b->rows * G, most = (double)b->max_rows * G, wide = c->head_dim == 128;
+    const double step = c->kv_heads * (rows / 16 + b->seqs / 2.0) * (b->max_ctx / 16.0) * (wide ? 0.65 : 0.46);
+    const double ctas = c->kv_heads * (rows / 256 + b->seqs / 2.0), tile = most <= 128 ? (wide ? 2400 : 2050) : (wide ? 3000 : 2500);
+    return std::max(1.0, ctas / sms) * (b->max_ctx / 128.0) * tile < step;
+}
+
 // The stream's places for the parts of items that a plan cuts, and their tickets.
 static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, uint32_t hd, Kv8StepPlan& p) {
     const size_t need = p.part_bytes(hd), tickets = (size_t)p.grid;
@@ -818,10 +830,10 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
     const int G = (int)(heads / c->kv_heads);
-    // Sequences of more rows than kPromptRows go to the tensor-memory kernel; a batch may hold both kinds,
-    // told apart on the device. All rows equal (or one sequence) means one kind.
+    // Sequences of more rows than kPromptRows go to the tensor-memory kernel, where the whole batch is worth it; a batch
+    // may hold both kinds, told apart on the device. All rows equal (or one sequence) means one kind.
     const long long most = (long long)b->max_rows * G;
-    const bool prompt = c->head_dim != 32 && q->dtype != POX_F32 && most > kPromptRows;
+    const bool prompt = c->head_dim != 32 && q->dtype != POX_F32 && most > kPromptRows && prompt_is_faster(c, b, G, ctx->num_sms);
     const bool step = !prompt || (b->seqs > 1 && b->rows != (unsigned long long)b->seqs * b->max_rows);
     Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, (int)c->head_dim, G, ctx->num_sms,
                                      prompt ? kPromptRows : 0x7fffffff);

@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
                         } else {
                             const float y0 = max3(y[0], y[1], y[2]), y1 = max3(y[3], y[4], y[5]), y2 = max3(y[6], y[7], y[8]),
                                         y3 = max3(y[9], y[10], y[11]), y4 = max3(y[12], y[13], y[14]);
-                            mx = fmaxf(mx, fmaf(max3(max3(y0, y1, y2), max3(y3, y4, y[15]), y0), f[g], pl[g]));
+                            mx = fmaxf(mx, fmaf(fmaxf(max3(y0, y1, y2), max3(y3, y4, y[15])), f[g], pl[g]));
                         }
                     }
                     if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
@@ -354,6 +354,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
             if (!bad) bad = !mbar_wait(full + 8 * (n % NST), (n / NST) & 1);
             tc_fence_after();
         };
+        auto release = [&](int n) {  // the stage, if the converters wait for it (nothing arrives there after the end)
+            if (n + NST < 2 * nk) umma_commit(empty + 8 * (n % NST));
+        };
         auto scores = [&](int t, int j) {
             const uint32_t k0 = kv + (2 * j % NST) * HB;
 #pragma unroll
@@ -375,17 +378,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
         wait_full(0);
         if (!bad) {
             for (int t = 0; t < nt; t++) scores(t, 0);
-            umma_commit(empty);
+            release(0);
         }
         for (int j = 0; j < nk && !bad; j++) {
             wait_full(2 * j + 1);
             for (int t = 0; t < nt && !bad; t++) {
                 values(t, j);
-                if (t == nt - 1) umma_commit(empty + 8 * ((2 * j + 1) % NST));
+                if (t == nt - 1) release(2 * j + 1);
                 if (j + 1 < nk) {
                     if (t == 0) wait_full(2 * j + 2);
                     if (!bad) scores(t, j + 1);
-                    if (t == nt - 1) umma_commit(empty + 8 * ((2 * j + 2) % NST));
+                    if (t == nt - 1) release(2 * j + 2);
                 }
             }
         }
