@@ -155,9 +155,10 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
         const uint32_t u1 = all <= x_end - x0 ? all : border(x_end - x0, all);
         if (u0 >= u1) continue;
         const int rows = sq.n * a.G, tiles = (rows + RT - 1) / RT;
+        auto token = [&](int row) { return sq.n == 1 ? 0 : row / a.G; };  // (of a valid row; a division costs a decode step)
         // tiles of a sequence in the order first, last, second, ..: early ones see fewer pages of a chunk
-        const int h = item / tiles, k_rt = item % tiles, rt = k_rt & 1 ? tiles - 1 - k_rt / 2 : k_rt / 2, row0 = rt * RT;
-        const int pos0 = sq.ctx - sq.n, pmin = pos0 + row0 / a.G, pmax = pos0 + (min(row0 + RT, rows) - 1) / a.G;
+        const int h = tiles == 1 ? (int)item : item / tiles, k_rt = item - h * tiles, rt = k_rt & 1 ? tiles - 1 - k_rt / 2 : k_rt / 2, row0 = rt * RT;
+        const int pos0 = sq.ctx - sq.n, pmin = pos0 + token(row0), pmax = pos0 + token(min(row0 + RT, rows) - 1);
         const int pages = pmax < 0 ? 0 : pmax / kPage + 1;
         const int page0 = max((int)u0 - kItemUnits, 0), page1 = min(pages, (int)u1 - kItemUnits);
         // the CTA that holds the item's first part, and the parts: one more than the borders that cut it
@@ -174,7 +175,8 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
         for (int n = 0; n < NT; n++) {
             const int row = row0 + 8 * n + g;
             const bool ok = row < rows;
-            const T* q = a.q.at((size_t)sq.r0 + (ok ? row / a.G : 0), h * a.G + (ok ? row % a.G : 0));
+            const int tk = ok ? token(row) : 0;
+            const T* q = a.q.at((size_t)sq.r0 + tk, h * a.G + (ok ? row - tk * a.G : 0));
 #pragma unroll
             for (int w = 0; w < KW; w++) {
                 const int d = HD == 32 ? 8 * t + 4 * w : 64 * (w / 4) + 16 * t + 4 * (w % 4);
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                 qf[n][e] = __shfl_sync(0xffffffffu, inv, 8 * t + 4 * e) * a.scale * (F32 ? 1.0f : 16777216.0f);
                 qo[n][e] = F32 ? 0.f : -kOffset * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
                 const int r = row0 + 8 * n + 2 * t + e;
-                rpos[n][e] = r < rows ? pos0 + r / a.G : 0;
+                rpos[n][e] = r < rows ? pos0 + token(r) : 0;
             }
         }
 
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
             if (ns == 1) {
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
                 const int row = row0 + r;
-                store4(a.out.at((size_t)sq.r0 + row / a.G, h * a.G + row % a.G) + d, a.vec,
+                store4(a.out.at((size_t)sq.r0 + token(row), h * a.G + row - token(row) * a.G) + d, a.vec,
                        make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
             } else {
                 float* y = part + (size_t)r * (HD + 2);
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
             }
             const float inv = L == 0.f ? 0.f : 1.0f / L;
             const int row = row0 + r;
-            store4(a.out.at((size_t)sq.r0 + row / a.G, h * a.G + row % a.G) + d, a.vec,
+            store4(a.out.at((size_t)sq.r0 + token(row), h * a.G + row - token(row) * a.G) + d, a.vec,
                    make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
         }
         }
