@@ -42,6 +42,10 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_here(float* v) {  // (no instruction: uses of v stay behind the wait)
     asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
 }
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+    const uint4 v = lds128(a);
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -60,7 +64,7 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 constexpr int kPromptKeys = 128;                   // tokens of a tile: 8 pages
 constexpr int kPromptThreads = 512;  // two softmax warpgroups, the converters, the MMA warp's group
 // registers of a thread of each group; the launch gives 128 to all, and these sum to as much
-constexpr int kSoftmaxRegs = 192, kConvertRegs = 96, kMmaRegs = 32;
+constexpr int kSoftmaxRegs = 184, kConvertRegs = 88, kMmaRegs = 56;
 static_assert(2 * kSoftmaxRegs + kConvertRegs + kMmaRegs <= 4 * 128, "more registers than the launch has");
 
 template <int HD>
@@ -88,6 +92,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
     constexpr uint32_t TS = 0, TO = 256;  // TMEM columns: S of tile t at 128 t, O at 256 + HD t
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * NST + 5];
+    __shared__ float4 scal[2][8];  // of a tile's pages: a, log2 b, 1 / b
     __shared__ uint32_t tmem_base;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -166,24 +171,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
         const int wpos = pos0 + (row0 + 32 * warp) / a.G;  // the first row of the warp sees no further
         float m = -INFINITY, ref = 0.f, l = 0.f;
         if (ti < nt) {
-            // lane i < 8 looks after page i of a tile: its entry two tiles ahead, its scales one tile ahead
-            auto entry = [&](int j) {
-                const int page = 8 * j + lane;
-                return lane < 8 && page <= last_page ? bt[page] : -1;
-            };
-            auto scales = [&](int blk, int j) {
-                if (blk < 0 || (uint32_t)blk >= a.c.num_blocks) {  // left out: u is -inf whatever S
-                    if (lane < 8 && 8 * j + lane <= last_page) atomicOr(a.err, kErrAttnPage);
-                    return make_float2(0.f, -1.f);
-                }
-                return *reinterpret_cast<const float2*>(a.c.scales + ((size_t)blk * a.c.kvh + h) * 2);
-            };
-            float2 ab = scales(entry(0), 0);
-            int next = entry(1);
             for (int j = 0; j < nk; j++) {
-                const float lb = ab.y == -1.f ? -INFINITY : log2f(fmaxf(ab.y, 1e-30f) + (ab.y - ab.y)),
-                            ib = ab.y == -1.f ? 0.f : 1.0f / fmaxf(ab.y, 1e-30f), ka = ab.x;
-                if (j + 1 < nk) ab = scales(next, j + 1), next = entry(j + 2);
+                // the pages' scalars come with V (whose stage is free again only when this tile's p has been used)
+                bad = __any_sync(0xffffffffu, !mbar_wait(full + 8 * ((2 * j + 1) % NST), ((2 * j + 1) / NST) & 1));
                 if (!bad) bad = __any_sync(0xffffffffu, !mbar_wait(sfull + 8 * ti, j & 1));
                 if (bad) break;
                 tc_fence_after();
@@ -191,10 +181,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
                 float x[kPromptKeys];
 #pragma unroll
                 for (int c = 0; c < 4; c++) tmem_ask32(ts + 32 * c, x + 32 * c);
-                float f[8], pl[8];  // u = S f + pl within a page
-#pragma unroll
-                for (int g = 0; g < 8; g++)
-                    f[g] = qf * __shfl_sync(0xffffffffu, ka, g), pl[g] = __shfl_sync(0xffffffffu, lb, g);
+                const uint32_t sc = smem_u32(scal[j & 1]);  // within a page u = S (qf a) + log2 b
                 tmem_wait_ld();
 #pragma unroll
                 for (int c = 0; c < 4; c++) tmem_here(x + 32 * c);
@@ -205,13 +192,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
 #pragma unroll
                     for (int g = 0; g < 8; g++) {
                         const float* y = x + 16 * g;
+                        const float4 pg = lds_f4(sc + 16 * g);
+                        const float f = qf * pg.x, pl = pg.y;
                         if (CUT) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) mx = fmaxf(mx, 16 * g + i > left ? -INFINITY : fmaf(y[i], f[g], pl[g]));
+                            for (int i = 0; i < 16; i++) mx = fmaxf(mx, 16 * g + i > left ? -INFINITY : fmaf(y[i], f, pl));
                         } else {
                             const float y0 = max3(y[0], y[1], y[2]), y1 = max3(y[3], y[4], y[5]), y2 = max3(y[6], y[7], y[8]),
                                         y3 = max3(y[9], y[10], y[11]), y4 = max3(y[12], y[13], y[14]);
-                            mx = fmaxf(mx, fmaf(fmaxf(max3(y0, y1, y2), max3(y3, y4, y[15])), f[g], pl[g]));
+                            mx = fmaxf(mx, fmaf(fmaxf(max3(y0, y1, y2), max3(y3, y4, y[15])), f, pl));
                         }
                     }
                     if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
@@ -235,8 +224,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
                         uint32_t hi[16];
 #pragma unroll
                         for (int g = 2 * c; g < 2 * c + 2; g++) {
-                            const float off = pl[g] - ref, pi = __shfl_sync(0xffffffffu, ib, g);
-                            const uint64_t f2 = pair2(f[g], f[g]), off2 = pair2(off, off);
+                            const float4 pg = lds_f4(sc + 16 * g);
+                            const float f = qf * pg.x, off = pg.y - ref;
+                            const uint64_t f2 = pair2(f, f), off2 = pair2(off, off);
                             uint64_t sum2 = 0;
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) {
@@ -250,7 +240,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
                                 hi[8 * (g & 1) + i / 2] = pack_f16(z.x, z.y);
                             }
                             const float sum = both(sum2).x + both(sum2).y;
-                            if (!CUT || sum != 0.f) l = fmaf(sum, pi, l);  // (an unseen page's scale may be anything)
+                            if (!CUT || sum != 0.f) l = fmaf(sum, pg.z, l);  // (an unseen page's scale may be anything)
                         }
                         tmem_st16(ts + 16 * c, hi);  // over columns of S
                     }
@@ -284,46 +274,63 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
         regs_less<kConvertRegs>();
         const int w = warp - 8, b = lane & 7, g = lane >> 3;
         constexpr int NI = HD / 16;  // 16-byte pieces of K (or V) per lane and tile
-        uint4 kr[NI], vr[NI];
-        auto page_at = [&](int j, int i) -> const int8_t* {
-            const int page = 8 * j + 2 * w + i, blk = page <= last_page ? bt[page] : -1;
-            return blk >= 0 && (uint32_t)blk < a.c.num_blocks ? a.c.pages + ((size_t)blk * a.c.kvh + h) * (32 * HD)
-                                                              : nullptr;
+        uint4 r[NI];  // K's pieces, then V's: the warps run ahead of the products, and more registers are the softmax's
+        // lane i looks after page i % 2 of the warp's two: its entry asked for two tiles ahead, its scales one
+        // (loads that every lane makes, looked at a tile later: behind a branch each tile began with their latency)
+        auto entry = [&](int j) { return bt[min(8 * j + 2 * w + (lane & 1), max(last_page, 0))]; };
+        auto there = [&](int blk, int j) {
+            const bool in = 8 * j + 2 * w + (lane & 1) <= last_page, ok = in && blk >= 0 && (uint32_t)blk < a.c.num_blocks;
+            if (in && !ok && lane < 2) atomicOr(a.err, kErrAttnPage);
+            return ok;
+        };
+        auto scales = [&](int blk, bool ok) {
+            return *reinterpret_cast<const float2*>(a.c.scales + ((size_t)(ok ? blk : 0) * a.c.kvh + h) * 2);
+        };
+        // (a page that is left out, or past the context, has p = 0: block 0 stands in for it, any bytes do)
+        auto page_of = [&](int blk, bool ok, int i) {
+            return a.c.pages + ((size_t)__shfl_sync(0xffffffffu, ok ? blk : 0, i) * a.c.kvh + h) * (32 * HD);
         };
         auto load_k = [&](const int8_t* p0, const int8_t* p1) {
 #pragma unroll
             for (int i = 0; i < NI; i++) {
                 const int8_t* p = i < NI / 2 ? p0 : p1;
                 const int q = i % (NI / 2), t = 8 * (q & 1) + b, c = 4 * (q >> 1) + g;
-                kr[i] = p ? ldg128_nc(p + kv8_k_off<HD>(t, 16 * c)) : make_uint4(0, 0, 0, 0);
+                r[i] = ldg128_nc(p + kv8_k_off<HD>(t, 16 * c));
             }
         };
         auto load_v = [&](const int8_t* p0, const int8_t* p1) {
 #pragma unroll
             for (int i = 0; i < NI; i++) {
                 const int8_t* p = i < NI / 2 ? p0 : p1;
-                vr[i] = p ? ldg128_nc(p + kv8_v_off<HD>(0, 32 * (i % (NI / 2)) + 8 * g + b)) : make_uint4(0, 0, 0, 0);
+                r[i] = ldg128_nc(p + kv8_v_off<HD>(0, 32 * (i % (NI / 2)) + 8 * g + b));
             }
         };
         auto put = [&](uint32_t at0, uint32_t at1, uint4 x) {
-            uint32_t r[8];
-            i8x4_to_f16x4(x.x, r[0], r[1]);
-            i8x4_to_f16x4(x.y, r[2], r[3]);
-            i8x4_to_f16x4(x.z, r[4], r[5]);
-            i8x4_to_f16x4(x.w, r[6], r[7]);
-            sts128(at0, r[0], r[1], r[2], r[3]);
-            sts128(at1, r[4], r[5], r[6], r[7]);
+            uint32_t f[8];
+            i8x4_to_f16x4(x.x, f[0], f[1]);
+            i8x4_to_f16x4(x.y, f[2], f[3]);
+            i8x4_to_f16x4(x.z, f[4], f[5]);
+            i8x4_to_f16x4(x.w, f[6], f[7]);
+            sts128(at0, f[0], f[1], f[2], f[3]);
+            sts128(at1, f[4], f[5], f[6], f[7]);
         };
         auto ready = [&](int st) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * st);
         };
-        const int8_t *p0 = page_at(0, 0), *p1 = page_at(0, 1);
+        int blk = nk ? entry(0) : 0, next = nk ? entry(1) : 0;
+        bool ok = there(blk, 0);
+        float2 ab = scales(blk, ok);
+        const int8_t *p0 = page_of(blk, ok, 0), *p1 = page_of(blk, ok, 1);
         if (nk) load_k(p0, p1);
         for (int j = 0; j < nk; j++) {
-            load_v(p0, p1);
-            if (j + 1 < nk) p0 = page_at(j + 1, 0), p1 = page_at(j + 1, 1);
+            // a page that is left out: u is -inf whatever S
+            const float4 sc = ok ? make_float4(ab.x, log2f(fmaxf(ab.y, 1e-30f) + (ab.y - ab.y)), 1.0f / fmaxf(ab.y, 1e-30f), 0.f)
+                                 : make_float4(0.f, -INFINITY, 0.f, 0.f);
+            blk = next, next = entry(j + 2);
+            ok = there(blk, j + 1);
+            ab = scales(blk, ok);
             int n = 2 * j, st = n % NST;
             if (n >= NST) bad = __any_sync(0xffffffffu, !mbar_wait(empty + 8 * st, (n / NST - 1) & 1));
             if (bad) break;
@@ -331,20 +338,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
             for (int i = 0; i < NI; i++) {
                 const int q = i % (NI / 2), t = 16 * (2 * w + i / (NI / 2)) + 8 * (q & 1) + b, c = 4 * (q >> 1) + g;
                 const uint32_t base = kv + st * HB + (c / 4) * (kPromptKeys * 128);
-                put(base + sw128_off(t, 2 * (c % 4)), base + sw128_off(t, 2 * (c % 4) + 1), kr[i]);
+                put(base + sw128_off(t, 2 * (c % 4)), base + sw128_off(t, 2 * (c % 4) + 1), r[i]);
             }
             ready(st);
-            if (j + 1 < nk) load_k(p0, p1);
+            load_v(p0, p1);
             n++, st = n % NST;
             if (n >= NST) bad = __any_sync(0xffffffffu, !mbar_wait(empty + 8 * st, (n / NST - 1) & 1));
             if (bad) break;
+            if (lane < 2) scal[j & 1][2 * w + lane] = sc;
 #pragma unroll
             for (int i = 0; i < NI; i++) {
                 const int page = 2 * w + i / (NI / 2), d = 32 * (i % (NI / 2)) + 8 * g + b;
                 const uint32_t base = kv + st * HB + (page / 4) * (HD * 128);
-                put(base + sw128_off(d, 2 * (page % 4)), base + sw128_off(d, 2 * (page % 4) + 1), vr[i]);
+                put(base + sw128_off(d, 2 * (page % 4)), base + sw128_off(d, 2 * (page % 4) + 1), r[i]);
             }
             ready(st);
+            p0 = page_of(blk, ok, 0), p1 = page_of(blk, ok, 1);
+            if (j + 1 < nk) load_k(p0, p1);
         }
     } else {  // ---- the products: one thread of warp 12
         regs_less<kMmaRegs>();
