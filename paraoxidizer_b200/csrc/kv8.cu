@@ -81,9 +81,9 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(QkArgs<T> a, int s
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, c = lane % L, nh = a.heads[0] + a.heads[1], rot = a.rope.rot;
     const unsigned long long item = (unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const uint32_t r = (uint32_t)(item / groups);
+    const uint32_t r = (uint32_t)div_u64(item, groups);
     if (r >= a.rows) return;
-    const int h0 = (int)(item % groups) * steps * HW + lane / L, turn = c < rot / (2 * V);
+    const int h0 = (int)(item - (unsigned long long)r * groups) * steps * HW + lane / L, turn = c < rot / (2 * V);
     const int d0 = turn ? c * V : 2 * c * V, d1 = turn ? rot / 2 + c * V : d0 + V;
     const T* src[2] = {a.in[0].at(r, 0), a.in[1].at(r, 0)};
     __shared__ uint4 ahead[kQkAhead][2][256];
@@ -213,12 +213,6 @@ struct AppendArgs {
     int* err;
 };
 
-// A page of the batch: sequence s owns page items (row_starts[s] + 30 s) / 16 .. (a bound of the pages that
-// its n rows touch: n rows reach at most (n + 30) / 16 pages, in closed form, so no scan over the sequences).
-__device__ __forceinline__ uint32_t page_base(const Kv8Batch& b, uint32_t s) {
-    return !b.row_starts ? s : (uint32_t)(((unsigned long long)b.row_starts[s] + 30ull * s) / 16);
-}
-
 // What a unit of the append and read kernels works on: one page of one kv head, k or v.
 struct PageUnit {
     SeqSpan sp;
@@ -228,17 +222,16 @@ struct PageUnit {
     int8_t* bytes;          // the page of the kv head
     float* scale;
 };
-// The unit of page item `item`, its entry loaded but not looked at; false (reported) if the batch is at fault.
-// W lanes work on the unit together. A sequence without a page of that number has first >= last.
-template <int W>
+// The unit of page item `item` (the warp's), its entry loaded but not looked at; false (reported) if the batch is at
+// fault. A sequence without a page of that number has first >= last.
 __device__ __forceinline__ bool page_unit(const Kv8Batch& b, uint32_t item, PageUnit& o, int* err) {
-    const uint32_t s = b.row_starts ? find_seq<W>(b, item, 30, 16) : item;
+    const uint32_t s = b.row_starts ? find_page_seq(b, item) : item;
     o.first = kPage, o.last = 0, o.page = 0, o.row = 0, o.blk = 0, o.bytes = nullptr;
     if (!seq_span(b, s, o.sp, err)) return false;
     const int begin = o.sp.ctx - o.sp.n, p0 = max(begin, 0);
     const int j = (int)(item - page_base(b, s));
     if (j < 0) {  // row_starts does not begin at 0
-        if (threadIdx.x % W == 0) atomicOr(err, kErrBatch);
+        atomicOr(err, kErrBatch);
         return false;
     }
     o.page = p0 / kPage + j;
@@ -291,17 +284,16 @@ enum { kTurnAny = 0, kTurnNone = 1, kTurnHalf = 2, kTurnPairs = 3 };
 // The page's new rows set the scale, its older slots follow if the scale grew. A lane's four dims make a word of
 // each K row and 8 bytes of each of four V rows.
 template <int HD, typename T, int TURN>
-__global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uint32_t items) {
+__global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uint32_t ctas) {
     constexpr int L = HD / 4, UC = 128 / (2 * L), NT = kPage / 2;
     pdl_wait();
     pdl_launch_dependents();
     __shared__ float red[4];
     const int lane = threadIdx.x & 31, c = threadIdx.x % L, hi = threadIdx.x / L & 1, t0 = NT * hi;
-    const unsigned long long u = (unsigned long long)blockIdx.x * UC + threadIdx.x / (2 * L);
-    const uint32_t item = min((uint32_t)(u / (2 * a.c.kvh)), items - 1);
-    const int h = (int)(u % a.c.kvh), side = (int)(u / a.c.kvh % 2);
+    const uint32_t item = blockIdx.x / ctas;
+    const int u = (blockIdx.x - item * ctas) * UC + threadIdx.x / (2 * L), side = u >= a.c.kvh, h = min(u - side * a.c.kvh, a.c.kvh - 1);
     PageUnit o;
-    bool live = page_unit<L>(a.b, item, o, a.err) && u < (unsigned long long)items * 2 * a.c.kvh && o.first < o.last;
+    bool live = page_unit(a.b, item, o, a.err) && u < 2 * a.c.kvh && o.first < o.last;
     const int rot = TURN == kTurnNone || side ? 0 : a.rope.rot, half = rot / 2, pos0 = o.page * kPage + t0;
     if (live && rot && (uint32_t)(o.page * kPage + o.last - 1) >= a.rope.positions) {
         if (c == 0) atomicOr(a.err, kErrRopePos);
@@ -481,17 +473,15 @@ __global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uin
 // The append's units the other way round, one group of HD / 4 lanes to all tokens of a unit. The unit of a sequence's first page also clears its padding rows.
 template <int HD, typename T>
 __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8Cache cache, Kv8Batch b, RowsView<T> k, RowsView<T> v,
-                                                       uint32_t items, int vec, int* err) {
-    constexpr int L = HD / 4, UW = 32 / L;
+                                                       uint32_t ctas, int vec, int* err) {
+    constexpr int L = HD / 4;
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, c = lane % L;
-    const unsigned long long u = ((unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * UW + lane / L;
-    const uint32_t item = min((uint32_t)(u / (2 * cache.kvh)), items - 1);
-    const int h = (int)(u % cache.kvh), side = (int)(u / cache.kvh % 2);
+    const uint32_t item = blockIdx.x / ctas;
+    const int c = threadIdx.x % L, u = (blockIdx.x - item * ctas) * (128 / L) + threadIdx.x / L, side = u >= cache.kvh,
+              h = u - side * cache.kvh;
     PageUnit o;
-    const bool ok = page_unit<L>(b, item, o, err);
-    if (!ok || u >= (unsigned long long)items * 2 * cache.kvh) return;
+    if (!page_unit(b, item, o, err) || u >= 2 * cache.kvh) return;
     const RowsView<T>& out = side ? v : k;
     const int begin = o.sp.ctx - o.sp.n;
     if (begin < 0 && o.page == 0)
@@ -607,13 +597,14 @@ constexpr int kPromptRows = 64;
 
 // Which of the attention's kernels a batch of more rows should take, from the bounds that the host knows. The step kernel
 // spreads rows by 16 and the context over the whole GPU, a page of a tile at about 0.65 ns (head dim 128; 64: 0.46); a CTA of
-// the prompt kernel walks the context for 256 rows, 128 tokens in 3.0 us (up to 128 rows 2.4; head dim 64: 2.5,
-// 2.05). Measured both ways: one sequence of 128 tokens x 4 heads at 4096 tokens, 8 kv heads of 128: 57 us against 98;
-// eight of them: 350 against 105; eight of 32 tokens: 101 against 82; at 32768 tokens one of 256: 578 against 625.
+// the prompt kernel walks the context for 256 rows, 128 tokens in 2.75 us (up to 128 rows 2.35; head dim 64: 2.35 and
+// 2.05). Both ways measured, bf16, 8 kv heads of 128 with 4 query heads each, step against prompt kernel: one sequence of
+// 128 rows at 4096 tokens 59 us against 90, of 512 at 512 43 against 31; eight of 32 rows at 4096 103 against 77, of 16 61
+// against 75; one of 256 at 32768 580 against 556.
 static bool prompt_is_faster(const pox_kv8_cache* c, const pox_kv8_batch* b, int G, int sms) {
     const double rows = (double)b->rows * G, most = (double)b->max_rows * G, wide = c->head_dim == 128;
     const double step = c->kv_heads * (rows / 16 + b->seqs / 2.0) * (b->max_ctx / 16.0) * (wide ? 0.65 : 0.46);
-    const double ctas = c->kv_heads * (rows / 256 + b->seqs / 2.0), tile = most <= 128 ? (wide ? 2400 : 2050) : (wide ? 3000 : 2500);
+    const double ctas = c->kv_heads * (rows / 256 + b->seqs / 2.0), tile = most <= 128 ? (wide ? 2350 : 2050) : (wide ? 2750 : 2350);
     return std::max(1.0, ctas / sms) * (b->max_ctx / 128.0) * tile < step;
 }
 
@@ -699,12 +690,13 @@ static cudaError_t launch_append(pox_cuda_ctx* ctx, const pox_kv8_cache* c, cons
                                  const pox_rows* v, const pox_rope* rope, cudaStream_t st) {
     AppendArgs<T> a{cache_view(c), batch_view(b), {rows_view<const T>(*k), rows_view<const T>(*v)}, rope_view(rope),
                     ctx->err_dev};
-    const uint32_t items = page_items(b);
-    const unsigned long long lanes = (unsigned long long)items * c->kv_heads * 2 * (HD / 2);
-    const unsigned grid = (unsigned)((lanes + 127) / 128);
+    constexpr unsigned kUnits = 128 / (HD / 2);  // of a CTA
+    const unsigned ctas = (2 * c->kv_heads + kUnits - 1) / kUnits;  // of a page item
+    const unsigned long long grid = (unsigned long long)page_items(b) * ctas;
+    if (grid > 0x7fffffffu) return cudaErrorInvalidConfiguration;
     const RopeView& r = a.rope;
     const bool vec = vec4(k) && vec4(v) && ((uintptr_t)r.table & 15) == 0;
-    auto go = [&](auto* kernel) { return launch_pdl(kernel, dim3(grid), dim3(128), 0, st, a, items); };
+    auto go = [&](auto* kernel) { return launch_pdl(kernel, dim3((unsigned)grid), dim3(128), 0, st, a, ctas); };
     return vec && !r.rot                      ? go(kv8_append_kernel<HD, T, kTurnNone>)
            : vec && r.half && r.rot % 8 == 0  ? go(kv8_append_kernel<HD, T, kTurnHalf>)
            : vec && !r.half && r.rot % 4 == 0 ? go(kv8_append_kernel<HD, T, kTurnPairs>)
@@ -714,10 +706,12 @@ static cudaError_t launch_append(pox_cuda_ctx* ctx, const pox_kv8_cache* c, cons
 template <int HD, typename T>
 static cudaError_t launch_read(pox_cuda_ctx* ctx, const pox_kv8_cache* c, const pox_kv8_batch* b, const pox_rows* k,
                                const pox_rows* v, cudaStream_t st) {
-    const uint32_t items = page_items(b);
-    const unsigned long long lanes = (unsigned long long)items * c->kv_heads * 2 * (HD / 4);
-    return launch_pdl(kv8_read_kernel<HD, T>, dim3((unsigned)((lanes + 127) / 128)), dim3(128), 0, st, cache_view(c),
-                      batch_view(b), rows_view<T>(*k), rows_view<T>(*v), items, vec4(k) && vec4(v), ctx->err_dev);
+    constexpr unsigned kUnits = 128 / (HD / 4);  // of a CTA
+    const unsigned ctas = (2 * c->kv_heads + kUnits - 1) / kUnits;
+    const unsigned long long grid = (unsigned long long)page_items(b) * ctas;
+    if (grid > 0x7fffffffu) return cudaErrorInvalidConfiguration;
+    return launch_pdl(kv8_read_kernel<HD, T>, dim3((unsigned)grid), dim3(128), 0, st, cache_view(c), batch_view(b),
+                      rows_view<T>(*k), rows_view<T>(*v), ctas, vec4(k) && vec4(v), ctx->err_dev);
 }
 
 // f.template operator()<HD, T>() for the head dim and the rows' type

@@ -93,18 +93,25 @@ __device__ __forceinline__ bool seq_span(const Kv8Batch& b, uint32_t s, SeqSpan&
     return true;
 }
 
-// The sequence of item i when sequence s owns the items f(s) .. f(s + 1) - 1, f(s) = (row_starts[s] + per_seq s) / div:
-// the largest s with f(s) <= i. Called by whole warps, each group of W lanes with an item of its own: W candidates
-// a round, so two dependent loads serve 1024 sequences at W = 32.
-template <int W>
-__device__ __forceinline__ uint32_t find_seq(const Kv8Batch& b, uint32_t i, uint32_t per_seq, uint32_t div) {
-    const uint32_t lane = threadIdx.x % W, shift = (threadIdx.x & 31) / W * W;
+// (a long division is a hundred instructions)
+__device__ __forceinline__ unsigned long long div_u64(unsigned long long a, uint32_t b) {
+    return a >> 32 ? a / b : (uint32_t)a / b;
+}
+
+// A page of the batch: sequence s owns page items (row_starts[s] + 30 s) / 16 .. (a bound of the pages that
+// its n rows touch: n rows reach at most (n + 30) / 16 pages, in closed form, so no scan over the sequences).
+__device__ __forceinline__ uint32_t page_base(const Kv8Batch& b, uint32_t s) {
+    return !b.row_starts ? s : (uint32_t)(((unsigned long long)b.row_starts[s] + 30ull * s) / 16);
+}
+
+// The sequence of page item i, the same for the warp: the largest s with page_base(s) <= i. 32 candidates a round, so
+// two dependent loads serve 1024 sequences.
+__device__ __forceinline__ uint32_t find_page_seq(const Kv8Batch& b, uint32_t i) {
+    const uint32_t lane = threadIdx.x & 31;
     uint32_t lo = 0, n = b.seqs;  // the answer is in [lo, lo + n)
-    while (__any_sync(0xffffffffu, n > 1)) {
-        const uint32_t step = (n + W - 1) / W, at = lane * step;
-        const bool le = at < n && ((unsigned long long)b.row_starts[lo + at] + (unsigned long long)per_seq * (lo + at)) / div <= i;
-        const uint32_t m = (__ballot_sync(0xffffffffu, le) >> shift) & (0xffffffffu >> (32 - W));
-        const uint32_t k = m ? 31 - __clz(m) : 0;
+    while (n > 1) {
+        const uint32_t step = (n + 31) / 32, at = lane * step;
+        const uint32_t m = __ballot_sync(0xffffffffu, at < n && page_base(b, lo + at) <= i), k = m ? 31 - __clz(m) : 0;
         lo += k * step;
         n = min(step, n - k * step);
     }
