@@ -415,8 +415,14 @@ int pox_cuda_kv8_read(pox_cuda_ctx* ctx, const pox_kv8_cache* cache, const pox_k
  * and sums are f32; f16 and bf16 rows enter the products exactly, f32 rows as pairs of f16 (22
  * bits); a row that sees nothing is 0. q and out: rows [batch->rows][heads] of one dtype. Sequences of few
  * rows split their context over the GPU and are joined in the same launch, in a fixed order: results do
- * not change from run to run. The first call on a stream, and one with larger sizes, allocates that
- * stream's split partials (held by the context): make it before capturing the stream. */
+ * not change from run to run. out must not overlap q. The first call on a stream allocates that stream's
+ * split partials (about 5 MB, held by the context, enough for all later calls): make it before capturing
+ * the stream. A captured call keeps to the partials of the stream that it was captured on, so its replays
+ * must not run beside other calls on that stream. A sequence has at most 2^30 rows times query heads of a
+ * kv head (else POX_ERR_UNSUPPORTED). A batch of sequences whose pages, counted once for each 16 such rows
+ * and kv head, sum to about 2^32 is refused on the device (POX_ERR_INVALID from the next
+ * pox_cuda_synchronize; f16 and bf16 prompts of head_dim 64 and 128 that are worth a CTA of their own do
+ * not count). */
 int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* cache, const pox_kv8_batch* batch, const pox_rows* q,
                            const pox_rows* out, uint32_t heads, float scale, void* stream);
 

@@ -47,9 +47,7 @@ namespace pox {
 // streams may overlap): the parts of items that are cut, and their tickets, zero between launches.
 struct Kv8Scratch {
     float* part = nullptr;
-    size_t part_bytes = 0;
-    uint32_t* tickets = nullptr;
-    size_t tickets_n = 0;
+    uint32_t* tickets = nullptr;  // behind the parts, once they are cleared
 };
 }  // namespace pox
 

@@ -66,13 +66,14 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(QkArgs<T> a) {
     for (int d = rot + lane; d < a.hd; d += 32) y[d] = from_f32<T>(val(d));
 }
 
-// Bound by HBM (each element once in, once out), by the launch for a few rows. 16 bytes a load: of the L = hd / (2 V)
-// lanes of a head (V elements in 16 bytes), lane c holds the V dims from c V and the V dims from rot / 2 + c V, so that both
-// kinds of pairs lie within a lane, and what is not rotated in order behind. A warp takes 32 / L heads of a row at once and
-// `steps` such groups of it and keeps the row's cosines and sines and the norm's weights meanwhile. kQkAhead groups are on
-// their way to shared memory, each lane's pieces to a place of its own (held in registers, two of them left too few
-// bytes in flight for HBM). All arithmetic goes two elements to an instruction: at one each, the issue slots
-// were as busy as the memory.
+// Bound by HBM (each element once in, once out): 16384 rows of 64 + 8 heads of 128, bf16, in 111 us, 84 % of the measured
+// copy rate. A few rows are bound by the launch: 4 us on the device up to some hundred rows.
+// 16 bytes a load: of the L = hd / (2 V) lanes of a head (V elements in 16 bytes), lane c holds the V dims from c V and
+// the V dims from rot / 2 + c V, so that both kinds of pairs lie within a lane, and what is not rotated in order behind.
+// A warp takes 32 / L heads of a row at once and `steps` such groups of it and keeps the row's cosines and sines and the
+// norm's weights meanwhile. kQkAhead groups are on their way to shared memory, each lane's pieces to a place of its own
+// (held in registers, two of them left too few bytes in flight for HBM). All arithmetic goes two elements to an
+// instruction: at one each, the issue slots were as busy as the memory.
 constexpr int kQkAhead = 4;
 template <typename T, int L, bool HALF>
 __global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(QkArgs<T> a, int steps, int groups) {
@@ -103,8 +104,8 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(QkArgs<T> a, int s
         if (lane == 0) atomicOr(a.err, kErrRopePos);
         return;
     }
-    // HALF: cosines and sines of the V pairs, two to a register pair. Else (cos, sin) and (-sin, cos) of each of them: the
-    // pairs of the lower piece, then of the upper one.
+    // HALF: cosines and sines of the V pairs, two to a register pair. Else (cos, sin) and (-sin, cos) of each of them:
+    // the pairs of the lower piece, then of the upper one.
     uint64_t cs[V], sn[HALF ? 1 : V];
     if (turn) {
         const float2* t = a.rope.table + (size_t)p * (rot / 2);
@@ -225,7 +226,7 @@ struct PageUnit {
 // The unit of page item `item` (the warp's), its entry loaded but not looked at; false (reported) if the batch is at
 // fault. A sequence without a page of that number has first >= last.
 __device__ __forceinline__ bool page_unit(const Kv8Batch& b, uint32_t item, PageUnit& o, int* err) {
-    const uint32_t s = b.row_starts ? find_page_seq(b, item) : item;
+    const uint32_t s = b.row_starts ? find_seq(b, item, [&](uint32_t q) { return page_base(b, q); }) : item;
     o.first = kPage, o.last = 0, o.page = 0, o.row = 0, o.blk = 0, o.bytes = nullptr;
     if (!seq_span(b, s, o.sp, err)) return false;
     const int begin = o.sp.ctx - o.sp.n, p0 = max(begin, 0);
@@ -278,20 +279,25 @@ __device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t 
 // four elements at once and turn pairs within a lane (interleaved) or between lanes (halves of whole lanes).
 enum { kTurnAny = 0, kTurnNone = 1, kTurnHalf = 2, kTurnPairs = 3 };
 
-// Bound by HBM: rows in once, bytes out once. A unit (page, kv head, side) is taken by two groups of HD / 4 lanes, lane c
-// of group `hi` on dims 4 c .. 4 c + 3 of tokens 8 hi .. 8 hi + 7, whose rows are all in flight at once (with all 16
-// tokens on a lane, 168 registers left 12 warps to an SM, and the loads' latency showed: 46 us for a 16381-token f32 prompt).
-// The page's new rows set the scale, its older slots follow if the scale grew. A lane's four dims make a word of
+// Rows in once, bytes out once: a 16381-token f32 prompt (8 kv heads of 128, 176 MB with the rotation's table) in 44 us,
+// 61 % of the measured copy rate: the chain of a unit (its rows, their turn, the maximum, the bytes) with 5 CTAs to an SM
+// to cover it, and the arithmetic beside it. A decode step (5 us on the device) and a ragged batch of 8000 rows (9.6)
+// are that chain once or a few times.
+// A unit (page, kv head, side) is taken by two groups of HD / 4 lanes, lane c of group `hi` on dims 4 c .. 4 c + 3 of
+// tokens 8 hi .. 8 hi + 7, whose rows are all in flight at once (with all 16 tokens on a lane, 168 registers left 12
+// warps to an SM: no faster; a loop over the heads that fetches ahead: 66 us). The page's new rows set the scale, its older slots follow if the scale grew. A lane's four dims make a word of
 // each K row and 8 bytes of each of four V rows.
 template <int HD, typename T, int TURN>
 __global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uint32_t ctas) {
     constexpr int L = HD / 4, UC = 128 / (2 * L), NT = kPage / 2;
     pdl_wait();
     pdl_launch_dependents();
+    if (check_batch(a.b, a.err)) return;
     __shared__ float red[4];
     const int lane = threadIdx.x & 31, c = threadIdx.x % L, hi = threadIdx.x / L & 1, t0 = NT * hi;
     const uint32_t item = blockIdx.x / ctas;
-    const int u = (blockIdx.x - item * ctas) * UC + threadIdx.x / (2 * L), side = u >= a.c.kvh, h = min(u - side * a.c.kvh, a.c.kvh - 1);
+    const int u = (blockIdx.x - item * ctas) * UC + threadIdx.x / (2 * L), side = u >= a.c.kvh,
+              h = min(u - side * a.c.kvh, a.c.kvh - 1);
     PageUnit o;
     bool live = page_unit(a.b, item, o, a.err) && u < 2 * a.c.kvh && o.first < o.last;
     const int rot = TURN == kTurnNone || side ? 0 : a.rope.rot, half = rot / 2, pos0 = o.page * kPage + t0;
@@ -330,8 +336,8 @@ __global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uin
             for (int i = 0; i < 4; i++) {
                 const int t = tc + i;
                 if (mine && in(t)) {
-                    const float4* q = reinterpret_cast<const float4*>(a.rope.table + (size_t)(pos0 + t) * half +
-                                                                      (TURN == kTurnHalf ? 4 * c - (low ? 0 : half) : 2 * c));
+                    const int at = TURN == kTurnHalf ? 4 * c - (low ? 0 : half) : 2 * c;
+                    const float4* q = reinterpret_cast<const float4*>(a.rope.table + (size_t)(pos0 + t) * half + at);
                     cs[i][0] = __ldg(q);
                     if (TURN == kTurnHalf) cs[i][1] = __ldg(q + 1);
                 }
@@ -438,7 +444,8 @@ __global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uin
                 uint32_t q[4];
                 quantise2(v[t][0], v[t][1], s2, r2, q[0], q[1]);
                 quantise2(v[t][2], v[t][3], s2, r2, q[2], q[3]);
-                *reinterpret_cast<uint32_t*>(o.bytes + kv8_k_off<HD>(t0 + t, 4 * c)) = pack_bytes(q[0], q[1], q[2], q[3]);
+                *reinterpret_cast<uint32_t*>(o.bytes + kv8_k_off<HD>(t0 + t, 4 * c)) =
+                    pack_bytes(q[0], q[1], q[2], q[3]);
             }
     } else if (whole || grew || (first < NT && last > 0)) {
 #pragma unroll
@@ -470,13 +477,16 @@ __global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uin
 }
 
 // ---- reading rows back -------------------------------------------------------------------------------
-// The append's units the other way round, one group of HD / 4 lanes to all tokens of a unit. The unit of a sequence's first page also clears its padding rows.
+// The append's units the other way round, one group of HD / 4 lanes to all tokens of a unit. The unit of a sequence's
+// first page also clears its padding rows. Bound by HBM: a 16381-token prompt (8 kv heads of
+// 128) to f32 rows, 168 MB, in 29 us, 88 % of the measured copy rate; a decode step by the launch, 5 us on the device.
 template <int HD, typename T>
 __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8Cache cache, Kv8Batch b, RowsView<T> k, RowsView<T> v,
                                                        uint32_t ctas, int vec, int* err) {
     constexpr int L = HD / 4;
     pdl_wait();
     pdl_launch_dependents();
+    if (check_batch(b, err)) return;
     const uint32_t item = blockIdx.x / ctas;
     const int c = threadIdx.x % L, u = (blockIdx.x - item * ctas) * (128 / L) + threadIdx.x / L, side = u >= cache.kvh,
               h = u - side * cache.kvh;
@@ -508,8 +518,9 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8Cache cache, Kv8Batch 
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const uint32_t q = side ? prmt(w[4 * e + t / 4], 0x4b000000u, 0x7440 + t % 4) : prmt(w[t], 0x4b000000u, 0x7440 + e);
                 // 2^23 + (byte + 128), exactly
+                const uint32_t q = side ? prmt(w[4 * e + t / 4], 0x4b000000u, 0x7440 + t % 4)
+                                        : prmt(w[t], 0x4b000000u, 0x7440 + e);
                 x[e] = __fmul_rn(__uint_as_float(q ^ 0x80u) - 8388736.0f, s);
             }
             store4(y + (size_t)(t - o.first) * out.row, vec, make_float4(x[0], x[1], x[2], x[3]));
@@ -527,7 +538,8 @@ static int check_rows(const pox_rows* r, const char* what, uint32_t rows, uint32
     // the farthest element's offset has to fit the address space with room to spare
     const unsigned __int128 far = (unsigned __int128)(rows ? rows - 1 : 0) * r->row_stride +
                                   (unsigned __int128)(heads ? heads - 1 : 0) * r->head_stride + hd;
-    if (far >= ((unsigned __int128)1 << 46)) return set_error(POX_ERR_INVALID, "%s: strides out of range", what);
+    if (far >= ((unsigned __int128)1 << 46))
+        return set_error(POX_ERR_INVALID, "%s: strides out of range", what);
     if (written) {
         const bool apart =
             ((heads <= 1 || r->head_stride >= hd) &&
@@ -553,7 +565,8 @@ static int check_rope(const pox_rope* r, uint32_t hd) {
 static RopeView rope_view(const pox_rope* r) {
     RopeView v{nullptr, 0, 0, 0};
     if (r && r->rot_dim)
-        v = RopeView{reinterpret_cast<const float2*>(r->table), r->positions, (int)r->rot_dim, r->style == POX_ROPE_HALF};
+        v = RopeView{reinterpret_cast<const float2*>(r->table), r->positions, (int)r->rot_dim,
+                     r->style == POX_ROPE_HALF};
     return v;
 }
 
@@ -589,48 +602,48 @@ static Kv8Cache cache_view(const pox_kv8_cache* c) {
 }
 static Kv8Batch batch_view(const pox_kv8_batch* b) {
     // as many rows as sequences and at most one each: one each, and no search on the device
-    return Kv8Batch{b->max_rows == 1 && b->rows == b->seqs ? nullptr : b->row_starts, b->ctx_lens, b->block_tables, b->seqs, b->rows, b->max_rows, b->max_ctx,
-                    b->max_blocks_per_seq};
+    const bool single = b->max_rows == 1 && b->rows == b->seqs;
+    return Kv8Batch{single ? nullptr : b->row_starts,   b->ctx_lens, b->block_tables,       b->seqs, b->rows,
+                    std::min(b->max_rows, b->rows), b->max_ctx,  b->max_blocks_per_seq};
 }
 
 constexpr int kPromptRows = 64;
 
-// Which of the attention's kernels a batch of more rows should take, from the bounds that the host knows. The step kernel
-// spreads rows by 16 and the context over the whole GPU, a page of a tile at about 0.65 ns (head dim 128; 64: 0.46); a CTA of
-// the prompt kernel walks the context for 256 rows, 128 tokens in 2.75 us (up to 128 rows 2.35; head dim 64: 2.35 and
-// 2.05). Both ways measured, bf16, 8 kv heads of 128 with 4 query heads each, step against prompt kernel: one sequence of
-// 128 rows at 4096 tokens 59 us against 90, of 512 at 512 43 against 31; eight of 32 rows at 4096 103 against 77, of 16 61
-// against 75; one of 256 at 32768 580 against 556.
+// Which of the attention's kernels a batch of more rows should take, from the bounds that the host knows. The step
+// kernel spreads rows by 16 and the context over the whole GPU, a page of a tile at about 0.65 ns (head dim 128; 64:
+// 0.46); a CTA of the prompt kernel walks the context for 256 rows, 128 tokens in 2.75 us (up to 128 rows 2.35; head dim
+// 64: 2.35 and 2.05). Both ways measured, bf16, 8 kv heads of 128 with 4 query heads each, step against prompt kernel:
+// one sequence of 128 rows at 4096 tokens 59 us against 90, of 512 at 512 43 against 31; eight of 32 rows at 4096 103
+// against 77, of 16 61 against 75; one of 256 at 32768 580 against 556.
 static bool prompt_is_faster(const pox_kv8_cache* c, const pox_kv8_batch* b, int G, int sms) {
-    const double rows = (double)b->rows * G, most = (double)b->max_rows * G, wide = c->head_dim == 128;
+    const double rows = (double)b->rows * G, most = (double)std::min(b->max_rows, b->rows) * G;
+    const bool wide = c->head_dim == 128;
     const double step = c->kv_heads * (rows / 16 + b->seqs / 2.0) * (b->max_ctx / 16.0) * (wide ? 0.65 : 0.46);
-    const double ctas = c->kv_heads * (rows / 256 + b->seqs / 2.0), tile = most <= 128 ? (wide ? 2350 : 2050) : (wide ? 2750 : 2350);
+    const double ctas = c->kv_heads * (rows / 256 + b->seqs / 2.0);
+    const double tile = most <= 128 ? (wide ? 2350 : 2050) : (wide ? 2750 : 2350);
     return std::max(1.0, ctas / sms) * (b->max_ctx / 128.0) * tile < step;
 }
 
-// The stream's places for the parts of items that a plan cuts, and their tickets.
-static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, uint32_t hd, Kv8StepPlan& p) {
-    const size_t need = p.part_bytes(hd), tickets = (size_t)p.grid;
+// The stream's places for the parts of items that a plan cuts, and their tickets: made by its first call, as large as any
+// plan on this device asks for, and kept as long as the context (a captured graph holds their addresses).
+static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, Kv8StepPlan& p) {
     try {
         std::lock_guard<std::mutex> lk(ctx->mu);
         Kv8Scratch& k = ctx->kv8[st];
-        if (need > k.part_bytes || tickets > k.tickets_n) {
+        if (!k.tickets) {
             cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
             if (cudaStreamIsCapturing(st, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone)
                 return set_error(POX_ERR_INVALID, "the parts' places must be allocated by a call before stream capture");
-            cudaError_t e = cudaStreamSynchronize(st);  // earlier calls may still use the old ones
-            if (e != cudaSuccess) return cuda_error(e, "cudaStreamSynchronize");
-            const size_t bytes = std::max(need, k.part_bytes), n = std::max(tickets, k.tickets_n);
-            cudaFree(k.part);
-            cudaFree(k.tickets);
-            k = Kv8Scratch();
-            e = cudaMalloc(&k.part, bytes);
-            if (e == cudaSuccess) k.part_bytes = bytes, e = cudaMalloc(&k.tickets, n * sizeof(uint32_t));
-            if (e == cudaSuccess) k.tickets_n = n, e = cudaMemsetAsync(k.tickets, 0, n * sizeof(uint32_t), st);
-            if (e != cudaSuccess) {
-                k.tickets_n = 0;  // so that the next call allocates and clears again
-                return cuda_error(e, "split partials");
+            const size_t tickets = (size_t)Kv8StepPlan::most_ctas(ctx->num_sms) * sizeof(uint32_t);
+            if (!k.part) {
+                const cudaError_t e = cudaMalloc(&k.part, Kv8StepPlan::most_part_bytes(ctx->num_sms) + tickets);
+                if (e != cudaSuccess) return cuda_error(e, "split partials");
             }
+            uint32_t* at = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(k.part) +
+                                                       Kv8StepPlan::most_part_bytes(ctx->num_sms));
+            const cudaError_t e = cudaMemsetAsync(at, 0, tickets, st);
+            if (e != cudaSuccess) return cuda_error(e, "split partials");
+            k.tickets = at;
         }
         p.part = k.part;
         p.tickets = k.tickets;
@@ -692,7 +705,7 @@ static cudaError_t launch_append(pox_cuda_ctx* ctx, const pox_kv8_cache* c, cons
                     ctx->err_dev};
     constexpr unsigned kUnits = 128 / (HD / 2);  // of a CTA
     const unsigned ctas = (2 * c->kv_heads + kUnits - 1) / kUnits;  // of a page item
-    const unsigned long long grid = (unsigned long long)page_items(b) * ctas;
+    const unsigned long long grid = (unsigned long long)page_items(b) * ctas + (a.b.row_starts ? 1 : 0);
     if (grid > 0x7fffffffu) return cudaErrorInvalidConfiguration;
     const RopeView& r = a.rope;
     const bool vec = vec4(k) && vec4(v) && ((uintptr_t)r.table & 15) == 0;
@@ -708,9 +721,10 @@ static cudaError_t launch_read(pox_cuda_ctx* ctx, const pox_kv8_cache* c, const 
                                const pox_rows* v, cudaStream_t st) {
     constexpr unsigned kUnits = 128 / (HD / 4);  // of a CTA
     const unsigned ctas = (2 * c->kv_heads + kUnits - 1) / kUnits;
-    const unsigned long long grid = (unsigned long long)page_items(b) * ctas;
+    const Kv8Batch view = batch_view(b);
+    const unsigned long long grid = (unsigned long long)page_items(b) * ctas + (view.row_starts ? 1 : 0);
     if (grid > 0x7fffffffu) return cudaErrorInvalidConfiguration;
-    return launch_pdl(kv8_read_kernel<HD, T>, dim3((unsigned)grid), dim3(128), 0, st, cache_view(c), batch_view(b),
+    return launch_pdl(kv8_read_kernel<HD, T>, dim3((unsigned)grid), dim3(128), 0, st, cache_view(c), view,
                       rows_view<T>(*k), rows_view<T>(*v), ctas, vec4(k) && vec4(v), ctx->err_dev);
 }
 
@@ -752,7 +766,8 @@ extern "C" int pox_cuda_qk_norm_rope(pox_cuda_ctx* ctx, const pox_qk_norm_rope* 
         if (rc) return rc;
         if (s.in->dtype != dtype || s.out->dtype != dtype)
             return set_error(POX_ERR_INVALID, "rows of different types (%s)", s.name);
-        if (s.in->data == s.out->data && (s.in->row_stride != s.out->row_stride || s.in->head_stride != s.out->head_stride))
+        if (s.in->data == s.out->data &&
+            (s.in->row_stride != s.out->row_stride || s.in->head_stride != s.out->head_stride))
             return set_error(POX_ERR_INVALID, "%s in place needs the same strides", s.name);
     }
     int rc = check_rope(&a->rope, a->head_dim);
@@ -767,7 +782,8 @@ extern "C" int pox_cuda_qk_norm_rope(pox_cuda_ctx* ctx, const pox_qk_norm_rope* 
     return e == cudaSuccess ? POX_OK : cuda_error(e, "qk_norm_rope launch");
 }
 
-static int check_kv_rows(const pox_kv8_cache* c, const pox_kv8_batch* b, const pox_rows* k, const pox_rows* v, bool written) {
+static int check_kv_rows(const pox_kv8_cache* c, const pox_kv8_batch* b, const pox_rows* k, const pox_rows* v,
+                         bool written) {
     int rc = check_rows(k, "k", b->rows, c->kv_heads, c->head_dim, written);
     if (!rc) rc = check_rows(v, "v", b->rows, c->kv_heads, c->head_dim, written);
     if (!rc && k->dtype != v->dtype) rc = set_error(POX_ERR_INVALID, "k and v rows of different types");
@@ -807,12 +823,14 @@ extern "C" int pox_cuda_kv8_read(pox_cuda_ctx* ctx, const pox_kv8_cache* c, cons
     return e == cudaSuccess ? POX_OK : cuda_error(e, "kv8_read launch");
 }
 
-extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c, const pox_kv8_batch* b, const pox_rows* q,
-                                      const pox_rows* out, uint32_t heads, float scale, void* stream) {
+extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c, const pox_kv8_batch* b,
+                                      const pox_rows* q, const pox_rows* out, uint32_t heads, float scale,
+                                      void* stream) {
     if (!ctx) return set_error(POX_ERR_INVALID, "ctx is NULL");
     int rc = check_cache(c, b);
     if (rc || b->rows == 0 || b->seqs == 0) return rc;
-    if (!heads || heads % c->kv_heads) return set_error(POX_ERR_INVALID, "%u heads over %u kv heads", heads, c->kv_heads);
+    if (!heads || heads % c->kv_heads)
+        return set_error(POX_ERR_INVALID, "%u heads over %u kv heads", heads, c->kv_heads);
     if (heads / c->kv_heads > 128)
         return set_error(POX_ERR_UNSUPPORTED, "%u query heads per kv head (at most 128)", heads / c->kv_heads);
     rc = check_rows(q, "q", b->rows, heads, c->head_dim, false);
@@ -824,15 +842,19 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     if (e != cudaSuccess) return cuda_error(e, "cudaSetDevice");
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
     const int G = (int)(heads / c->kv_heads);
+    const long long most = (long long)std::min(b->max_rows, b->rows) * G;
+    if (most > 1 << 30)  // (the kernels count a sequence's rows in int)
+        return set_error(POX_ERR_UNSUPPORTED, "%u rows of %d query heads", std::min(b->max_rows, b->rows), G);
     // Sequences of more rows than kPromptRows go to the tensor-memory kernel, where the whole batch is worth it; a batch
     // may hold both kinds, told apart on the device. All rows equal (or one sequence) means one kind.
-    const long long most = (long long)b->max_rows * G;
-    const bool prompt = c->head_dim != 32 && q->dtype != POX_F32 && most > kPromptRows && prompt_is_faster(c, b, G, ctx->num_sms);
+    const bool prompt = c->head_dim != 32 && q->dtype != POX_F32 && most > kPromptRows &&
+                        kv8_prompt_grid(batch_view(b), (int)c->kv_heads, G) <= 0x7fffffffu &&
+                        prompt_is_faster(c, b, G, ctx->num_sms);
     const bool step = !prompt || (b->seqs > 1 && b->rows != (unsigned long long)b->seqs * b->max_rows);
     Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, (int)c->head_dim, G, ctx->num_sms,
                                      prompt ? kPromptRows : 0x7fffffff);
     plan.device = ctx->device;
-    rc = step ? kv8_scratch(ctx, st, c->head_dim, plan) : POX_OK;
+    rc = step ? kv8_scratch(ctx, st, plan) : POX_OK;
     if (rc) return rc;
     const int vec = vec4(q) && vec4(out);
     e = by_shape(c->head_dim, q->dtype, [&](auto hd, auto t) {

@@ -104,14 +104,24 @@ __device__ __forceinline__ uint32_t page_base(const Kv8Batch& b, uint32_t s) {
     return !b.row_starts ? s : (uint32_t)(((unsigned long long)b.row_starts[s] + 30ull * s) / 16);
 }
 
-// The sequence of page item i, the same for the warp: the largest s with page_base(s) <= i. 32 candidates a round, so
-// two dependent loads serve 1024 sequences.
-__device__ __forceinline__ uint32_t find_page_seq(const Kv8Batch& b, uint32_t i) {
+// Items of a ragged batch are found through row_starts, where a sequence of fewer than no rows has none: the last CTA
+// looks at every sequence instead (true), so that each one at fault is reported.
+__device__ __forceinline__ bool check_batch(const Kv8Batch& b, int* err) {
+    if (!b.row_starts || blockIdx.x != gridDim.x - 1) return false;
+    SeqSpan q;
+    for (uint32_t s = threadIdx.x; s < b.seqs; s += blockDim.x) seq_span(b, s, q, err);
+    return true;
+}
+
+// The sequence of item i, the same for the warp: the largest s with base(s) <= i. 32 candidates a round, so two
+// dependent loads serve 1024 sequences.
+template <typename F>
+__device__ __forceinline__ uint32_t find_seq(const Kv8Batch& b, uint32_t i, F&& base) {
     const uint32_t lane = threadIdx.x & 31;
     uint32_t lo = 0, n = b.seqs;  // the answer is in [lo, lo + n)
     while (n > 1) {
         const uint32_t step = (n + 31) / 32, at = lane * step;
-        const uint32_t m = __ballot_sync(0xffffffffu, at < n && page_base(b, lo + at) <= i), k = m ? 31 - __clz(m) : 0;
+        const uint32_t m = __ballot_sync(0xffffffffu, at < n && base(lo + at) <= i), k = m ? 31 - __clz(m) : 0;
         lo += k * step;
         n = min(step, n - k * step);
     }

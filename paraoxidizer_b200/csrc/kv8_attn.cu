@@ -51,14 +51,15 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 }
 
 // The work of a launch is a line of units: for each sequence in turn, for each kv head and tile of 8 NT rows,
-// kItemUnits for starting on it and one for each page of the sequence. Every CTA takes an equal run of the line, whatever
-// the lengths are (with a CTA per split of the longest context, a quarter of the SMs' time went by idle at three sequences
-// of 131k, 109k and 61k tokens). A long item that a run's end cuts leaves its part in the CTA's place (0: of an item
-// begun before, 1: of one that goes on), and the CTA that comes last joins them in order.
+// kItemUnits for starting on it and one for each page of the sequence. Every CTA takes an equal run of the line,
+// whatever the lengths are (with a CTA per split of the longest context, 122 us against 106 at three sequences of 131k,
+// 109k and 61k tokens: a quarter of the SMs' time went by idle). A long item that a run's
+// end cuts leaves its part in the CTA's place (0: of an item begun before, 1: of one that goes on), and the CTA that
+// comes last joins them in order.
 //
-// Within an item each warp streams whole pages (K and V of 16 tokens of the kv head, 32 HD contiguous bytes) through a ring of
-// its own with one bulk copy a page, two pages a turn, and runs both products transposed on mma.sync m16n8k16 with f32
-// accumulators, so that a page is the 16 rows of A and 8 query rows fill N:
+// Within an item each warp streams whole pages (K and V of 16 tokens of the kv head, 32 HD contiguous bytes) through a
+// ring of its own with one bulk copy a page, two pages a turn, and runs both products transposed on mma.sync m16n8k16
+// with f32 accumulators, so that a page is the 16 rows of A and 8 query rows fill N:
 //   S^T (tokens x rows) = K Q^T,   O^T (dims x rows) = V^T P^T.
 // The MMA does not care in which order k and the rows of A run, so they run as the page's bytes lie: lane (g, t) takes
 // 16 dims of the tokens 4 (g / 2) + g % 2 (+ 2) for the first product and the four tokens 4 t .. 4 t + 3 of a dim for
@@ -66,6 +67,12 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 // f32 rows: q and p as two f16 terms each (22 bits), bytes converted exactly. 16-bit rows: q exact, bytes with the
 // offset of bytes_to_f16; p two terms for f16 outputs of up to 8 rows (so that only the output's own rounding
 // remains), one for bf16 and for more rows (2^-11 of p).
+//
+// What bounds it: HBM where the contexts are long (64 sequences of 3800 to 4400 tokens, 64 heads over 8 of 128, bf16:
+// 541 MB in 97 us, 85 % of the measured copy rate; the three above 106 us, 83 %); the start and joining of items
+// where there are many short ones (37 sequences of up to 2011 tokens, 12 heads of 64: 24 us, its bytes 8.4); for f32
+// rows the products of two terms each (20 prompts of up to 257 rows, 14 heads over 2 of 64: 120 us, mma.sync pipe 40 %
+// and issue slots 45 % busy at the 8 warps that the registers leave an SM); one sequence of 640 tokens the launch (5.6).
 constexpr uint32_t kWholePages = 128;
 
 template <int HD, typename T, int NT>
@@ -93,7 +100,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
         if (s >= a.b.seqs || !seq_span(a.b, s, q, a.err)) return 0;
         const int rows = q.n * a.G;
         if (rows > p.most_rows) return 0;
-        return (unsigned long long)(a.c.kvh * ((rows + RT - 1) / RT)) * (kItemUnits + max((q.ctx + kPage - 1) / kPage, 1));
+        return (unsigned long long)a.c.kvh * ((rows + RT - 1) / RT) * (kItemUnits + max((q.ctx + kPage - 1) / kPage, 1));
     };
     SeqSpan sq;
     const unsigned long long mine = units(lane, sq);
@@ -155,9 +162,10 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
         const uint32_t u1 = all <= x_end - x0 ? all : border(x_end - x0, all);
         if (u0 >= u1) continue;
         const int rows = sq.n * a.G, tiles = (rows + RT - 1) / RT;
-        auto token = [&](int row) { return sq.n == 1 ? 0 : row / a.G; };  // (of a valid row; a division costs a decode step)
+        auto token = [&](int row) { return sq.n == 1 ? 0 : row / a.G; };  // of a valid row
         // tiles of a sequence in the order first, last, second, ..: early ones see fewer pages of a chunk
-        const int h = tiles == 1 ? (int)item : item / tiles, k_rt = item - h * tiles, rt = k_rt & 1 ? tiles - 1 - k_rt / 2 : k_rt / 2, row0 = rt * RT;
+        const int h = tiles == 1 ? (int)item : item / tiles, k_rt = item - h * tiles;
+        const int row0 = (k_rt & 1 ? tiles - 1 - k_rt / 2 : k_rt / 2) * RT;
         const int pos0 = sq.ctx - sq.n, pmin = pos0 + token(row0), pmax = pos0 + token(min(row0 + RT, rows) - 1);
         const int pages = pmax < 0 ? 0 : pmax / kPage + 1;
         const int page0 = max((int)u0 - kItemUnits, 0), page1 = min(pages, (int)u1 - kItemUnits);
@@ -281,7 +289,8 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
 #pragma unroll
             for (int j = 0; j < NJ; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; e++) m[n][e] = -INFINITY, ref[n][e] = 0.f, l[n][e] = 0.f, ps[n][e] = ps[n][2 + e] = 0.f;
+            for (int e = 0; e < 2; e++)
+                m[n][e] = -INFINITY, ref[n][e] = 0.f, l[n][e] = 0.f, ps[n][e] = ps[n][2 + e] = 0.f;
         }
         const int tok = 4 * (g >> 1) + (g & 1);
         const uint32_t k_at = HD == 32 ? tok * HD + 8 * t : tok * HD + 16 * t, swap = HD == 128 ? (g & 1) << 6 : 0,
@@ -325,7 +334,8 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                     bytes_to_f16<F32>(kw[1][w], a1, a3);
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        if (w == 0) mma_start(u[k][n], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1], qo[n][0], qo[n][1]);
+                        if (w == 0)
+                            mma_start(u[k][n], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1], qo[n][0], qo[n][1]);
                         else mma_16816(u[k][n], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1]);
                         if constexpr (F32) mma_16816(u[k][n], a0, a1, a2, a3, qb[n][F32][w][0], qb[n][F32][w][1]);
                     }
@@ -398,7 +408,8 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                     }
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        // (p in f32: a page's p may be nothing in f16 next to its part of l. An unseen page's scale may be anything.)
+                        // (p in f32: a page's p may be nothing in f16 next to its part of l. An unseen page's scale may
+                        // be anything.)
                         const float y = x[e] + x[2 + e];
                         if (open || y != 0.f) l[n][e] = fmaf(y, pi[k], l[n][e]);
                     }
@@ -496,29 +507,29 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
         }
         if (last) {
             __threadfence();
-        for (int i = tid; i < valid * (HD / 4); i += 32 * kStepWarps) {
-            const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
-            float M = -INFINITY, L = 0.f;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = tid; i < valid * (HD / 4); i += 32 * kStepWarps) {
+                const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
+                float M = -INFINITY, L = 0.f;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-            for (uint32_t k = 0; k < ns; k++) {
-                const float* y = p.part + ((size_t)(2 * (c0 + k) + (k == 0)) * RT + r) * (HD + 2);
-                const float2 w = __ldcg(reinterpret_cast<const float2*>(y));
-                const float2 u = __ldcg(reinterpret_cast<const float2*>(y + 2 + d)),
-                             v = __ldcg(reinterpret_cast<const float2*>(y + 4 + d));
-                const float to = fmaxf(M, w.x);
-                const float fo = M == -INFINITY ? (L == 0.f ? 0.f : 1.f) : ex2(M - to),
-                            fn = w.x == -INFINITY ? (w.y == 0.f ? 0.f : 1.f) : ex2(w.x - to);
-                M = to;
-                L = fmaf(L, fo, w.y * fn);
-                x.x = fmaf(x.x, fo, u.x * fn), x.y = fmaf(x.y, fo, u.y * fn);
-                x.z = fmaf(x.z, fo, v.x * fn), x.w = fmaf(x.w, fo, v.y * fn);
+                for (uint32_t k = 0; k < ns; k++) {
+                    const float* y = p.part + ((size_t)(2 * (c0 + k) + (k == 0)) * RT + r) * (HD + 2);
+                    const float2 w = __ldcg(reinterpret_cast<const float2*>(y));
+                    const float2 u = __ldcg(reinterpret_cast<const float2*>(y + 2 + d)),
+                                 v = __ldcg(reinterpret_cast<const float2*>(y + 4 + d));
+                    const float to = fmaxf(M, w.x);
+                    const float fo = M == -INFINITY ? (L == 0.f ? 0.f : 1.f) : ex2(M - to),
+                                fn = w.x == -INFINITY ? (w.y == 0.f ? 0.f : 1.f) : ex2(w.x - to);
+                    M = to;
+                    L = fmaf(L, fo, w.y * fn);
+                    x.x = fmaf(x.x, fo, u.x * fn), x.y = fmaf(x.y, fo, u.y * fn);
+                    x.z = fmaf(x.z, fo, v.x * fn), x.w = fmaf(x.w, fo, v.y * fn);
+                }
+                const float inv = L == 0.f ? 0.f : 1.0f / L;
+                const int row = row0 + r;
+                store4(a.out.at((size_t)sq.r0 + token(row), h * a.G + row - token(row) * a.G) + d, a.vec,
+                       make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
             }
-            const float inv = L == 0.f ? 0.f : 1.0f / L;
-            const int row = row0 + r;
-            store4(a.out.at((size_t)sq.r0 + token(row), h * a.G + row - token(row) * a.G) + d, a.vec,
-                   make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-        }
         }
         fence_proxy_async_smem();  // the ring's space goes back to the copies
         __syncthreads();

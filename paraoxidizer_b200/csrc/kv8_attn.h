@@ -9,9 +9,10 @@
 
 namespace pox {
 
-constexpr int kStepWarps = 4;   // warps of a CTA of the step kernel
-constexpr int kItemUnits = 8;   // what an item of it costs besides its pages, in pages (8, 16, 32: 20.9, 21.0, 22.2 us
-                                // for 128 sequences of 50 to 3000 tokens; long contexts do not mind)
+constexpr int kStepWarps = 4;  // warps of a CTA of the step kernel
+// What an item of it costs besides its pages, in pages (8, 16, 32: 20.9, 21.0, 22.2 us for 128 sequences of 50 to 3000
+// tokens; long contexts do not mind).
+constexpr int kItemUnits = 8;
 
 template <typename T>
 struct Kv8Attn {
@@ -34,7 +35,13 @@ struct Kv8StepPlan {
     int device = 0;
     float* part = nullptr;        // [grid][2][8 tiles][hd + 2]
     uint32_t* tickets = nullptr;  // [grid], zero between launches
-    size_t part_bytes(uint32_t hd) const { return (size_t)grid * 2 * 8 * tiles * (hd + 2) * sizeof(float); }
+    // Bounds over all plans: CTAs of an SM, and the two places of each times its rows times their floats.
+    static constexpr int kNarrow = 4, kWide = 3, kTwoTiles = 2;
+    static int most_ctas(int sms) { return kNarrow * sms; }
+    static size_t most_part_bytes(int sms) {
+        return (size_t)sms * 2 * sizeof(float) *
+               std::max({kNarrow * 8 * (64 + 2), kWide * 8 * (128 + 2), kTwoTiles * 16 * (128 + 2)});
+    }
 };
 
 inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int hd, int G, int sms, int most_rows) {
@@ -47,7 +54,7 @@ inline Kv8StepPlan kv8_step_plan(const Kv8Batch& b, int kvh, int hd, int G, int 
     const long long items = (long long)b.seqs * kvh * ((rows + 8 * p.tiles - 1) / (8 * p.tiles));
     const long long pages = std::max<long long>((b.max_ctx + kPage - 1) / kPage, 1);
     const long long most = (long long)std::min((double)items * (pages + kItemUnits) / p.min_units + 1, 1e9);
-    p.grid = (int)std::min<long long>((p.tiles == 1 ? (hd == 128 ? 3 : 4) : 2) * sms, most);
+    p.grid = (int)std::min<long long>((p.tiles > 1 ? p.kTwoTiles : hd == 128 ? p.kWide : p.kNarrow) * sms, most);
     return p;
 }
 
@@ -64,6 +71,11 @@ inline cudaError_t kv8_smem_once(F* kernel, int bytes, int device, std::atomic<u
 // Sequences of at most p.most_rows rows (tokens times query heads of the group), any head dim.
 template <int HD, typename T>
 cudaError_t launch_kv8_step(const Kv8Attn<T>& a, const Kv8StepPlan& p, cudaStream_t st);
+// CTAs of the prompt kernel: one for each tile item and kv head, and the one that checks the batch.
+inline unsigned long long kv8_prompt_grid(const Kv8Batch& b, int kvh, int G) {
+    return b.row_starts ? ((unsigned long long)b.rows * G + 255ull * b.seqs) / 256 * kvh + 1
+                        : (unsigned long long)b.seqs * kvh;
+}
 // Sequences of at least min_rows rows, head dims 64 and 128, f16 and bf16.
 template <int HD, typename T>
 cudaError_t launch_kv8_prompt(const Kv8Attn<T>& a, int min_rows, int device, cudaStream_t st);

@@ -143,10 +143,7 @@ extern "C" void pox_cuda_destroy(pox_cuda_ctx* ctx) {
         cudaFree(ctx->tc_scratch);
         cudaFree(ctx->tc_tickets);
         cudaFree(ctx->attn_scratch);
-        for (auto& k : ctx->kv8) {
-            cudaFree(k.second.part);
-            cudaFree(k.second.tickets);
-        }
+        for (auto& k : ctx->kv8) cudaFree(k.second.part);
         cudaFreeHost(ctx->err_host);
         cudaStreamDestroy(ctx->stream);
     }

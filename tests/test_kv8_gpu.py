@@ -570,3 +570,65 @@ def test_bad_input_on_the_device_is_left_out_and_reported(be):
     with pytest.raises(L.PoxError, match="bounds"):
         be.synchronize()
     assert bool((out == 5.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_row_starts_that_descend_are_reported(be, dtype):
+    """A sequence of fewer than no rows owns no work, and is reported all the same; the others are computed."""
+    dt = TYPES[dtype][0]
+    ctx = [300, 300, 300]
+    c = Cache(ctx, 1, 64, seed=3)
+    b = c.batch([0, 300, 150, 450], ctx)
+    b.max_rows = 300
+    q, out = (torch.randn(450, 4, 64, device="cuda").to(dt) for _ in range(2))
+    kv = torch.randn(450, 1, 64, device="cuda").to(dt)
+    for call in (lambda: be.kv8_append(c.c, b, rows_of(kv), rows_of(kv), None, STREAM),
+                 lambda: be.kv8_read(c.c, b, rows_of(kv), rows_of(kv.clone()), STREAM),
+                 lambda: be.kv8_attention(c.c, b, rows_of(q), rows_of(out), 4, 0.0, STREAM)):
+        call()
+        with pytest.raises(L.PoxError, match="bounds"):
+            be.synchronize()
+    assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attention_of_a_prompt_among_single_tokens(be, dtype):
+    """One prompt among many decoding sequences, with a bound of the rows that says nothing."""
+    n = [1] * 21 + [700] + [1] * 33 + [0, 300]
+    ctx = [1 + 7 * i for i in range(21)] + [900] + [16 * i + 1 for i in range(33)] + [5, 300]
+    starts = [0]
+    for i in n:
+        starts.append(starts[-1] + i)
+    c = Cache(ctx, 2, 128, seed=4)
+    batch = c.batch
+
+    def loose(*a):
+        b = batch(*a)
+        b.max_rows = 2 ** 31
+        return b
+
+    c.batch = loose
+    check_attention(be, c, starts, ctx, 8, dtype)
+
+
+def test_a_graph_outlives_larger_calls_on_its_stream(be):
+    st = torch.cuda.Stream()
+    small, ctx = Cache([900], 2, 64, seed=5), [100 + 31 * i for i in range(70)]
+    large = Cache(ctx, 4, 128, seed=6)
+    bs, bl = small.batch([0, 1], [900]), large.batch(list(range(71)), ctx)
+    q, out = torch.randn(1, 4, 64, device="cuda"), torch.empty(1, 4, 64, device="cuda")
+    ql, outl = (torch.randn(70, 64, 128, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    be.kv8_attention(small.c, bs, rows_of(q), rows_of(out), 4, 0.0, st.cuda_stream)
+    torch.cuda.synchronize()
+    want = out.clone()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=st):
+        be.kv8_attention(small.c, bs, rows_of(q), rows_of(out), 4, 0.0, st.cuda_stream)
+    be.kv8_attention(large.c, bl, rows_of(ql), rows_of(outl), 64, 0.0, st.cuda_stream)
+    torch.cuda.synchronize()
+    out.zero_()
+    with torch.cuda.stream(st):
+        gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
