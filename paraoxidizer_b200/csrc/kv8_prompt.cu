@@ -91,7 +91,7 @@ struct PromptSmem {
 // f16 (2^-11 of p, as f16 and bf16 outputs are rounded to no more), the sums of p and O are f32. f32 rows stay with the
 // step kernel: carried as two f16 terms through these products, an output was 7e-6 off (the tensor core drops low bits
 // as it adds up) where mma.sync is 3e-7 off.
-// 8192 rows over themselves, 32 heads over 8 of 128, bf16: 629 to 658 us, 870 to 835 TFLOP/s, 53 % of the measured rate
+// 8192 rows over themselves, 32 heads over 8 of 128, bf16: 632 us, 870 TFLOP/s, 53 % of the measured rate
 // of library products. The round trip of a tile bounds it: a row tile's next product waits for its softmax, and the
 // two softmaxes together take longer than the products that they hide (tensor pipe 38 % busy, exponentials 38 %).
 // An MMA completes in order with those issued before it: S of tile j ready means P V of tile j - 1 done.
@@ -124,6 +124,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
     const int rows = sq.n * a.G, k_tile = a.b.row_starts ? (int)(item - first_item(s)) : 0;
     const int row0 = ((rows + 255) / 256 - 1 - k_tile) * 256;
     if (rows < min_rows || k_tile < 0 || row0 < 0) return;
+    // (what the outputs' addresses are made of waits in shared memory: in registers it made the softmax spill, 722 us
+    // against 632)
+    __shared__ uint32_t place_s[2];
+    if (tid == 0) place_s[0] = row0, place_s[1] = sq.r0;
     const int pos0 = sq.ctx - sq.n, pmax = pos0 + (min(row0 + 256, rows) - 1) / a.G;
     const int nt = row0 + 128 < rows ? 2 : 1, nk = pmax < 0 ? 0 : pmax / kPromptKeys + 1;
     const int32_t* bt = a.b.btab + (size_t)s * a.b.mbps;
@@ -272,7 +276,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
             if (nk && !bad) bad = __any_sync(0xffffffffu, !mbar_wait(ofull, 0));
             tc_fence_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l;
-            T* y = a.out.at((size_t)sq.r0 + (mine ? row / a.G : 0), h * a.G + (mine ? row % a.G : 0));
+            const volatile uint32_t* place = place_s;
+        const int last_row = (int)place[0] + tid;
+        T* y = a.out.at((size_t)place[1] + (mine ? last_row / a.G : 0), h * a.G + (mine ? last_row % a.G : 0));
 #pragma unroll
             for (int c = 0; c < HD / 32; c++) {
                 float x[32];
