@@ -864,7 +864,7 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
         constexpr int HD = decltype(hd)::value;
         cudaError_t r = cudaSuccess;
         if constexpr (HD != 32 && sizeof(T) == 2)
-            if (prompt) r = launch_kv8_prompt<HD, T>(a, kPromptRows + 1, ctx->device, st);
+            if (prompt) r = launch_kv8_prompt<HD, T>(a, step ? kPromptRows + 1 : 1, ctx->device, st);
         if (r == cudaSuccess && step) r = launch_kv8_step<HD, T>(a, plan, st);
         return r;
     });

@@ -93,7 +93,7 @@ struct PromptSmem {
 // as it adds up) where mma.sync is 3e-7 off.
 // 8192 rows over themselves, 32 heads over 8 of 128, bf16: 632 us, 870 TFLOP/s, 53 % of the measured rate
 // of library products. The round trip of a tile bounds it: a row tile's next product waits for its softmax, and the
-// two softmaxes together take longer than the products that they hide (tensor pipe 38 % busy, exponentials 38 %).
+// two softmaxes together take longer than the products that they hide (tensor pipe 40 % busy, exponentials 41 %).
 // An MMA completes in order with those issued before it: S of tile j ready means P V of tile j - 1 done.
 template <int HD, typename T>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8Attn<T> a, int min_rows) {

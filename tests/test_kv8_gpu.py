@@ -632,3 +632,13 @@ def test_a_graph_outlives_larger_calls_on_its_stream(be):
         gr.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def test_attention_refuses_more_rows_than_it_counts(be):
+    c = Cache([16], 1, 64, seed=7)
+    q = torch.zeros(1, 128, 64, device="cuda")
+    b = c.batch([0, 1], [16])
+    b.row_starts, b.rows, b.max_rows = c.keep[0].data_ptr(), 2 ** 24, 2 ** 24
+    with pytest.raises(L.PoxError) as e:
+        be.kv8_attention(c.c, b, rows_of(q), rows_of(torch.empty_like(q)), 128, 0.0, STREAM)
+    assert e.value.code == L.POX_ERR_UNSUPPORTED
