@@ -71,7 +71,7 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 // What bounds it: HBM where the contexts are long (64 sequences of 3800 to 4400 tokens, 64 heads over 8 of 128, bf16:
 // 541 MB in 97 us, 85 % of the measured copy rate; the three above 106 us, 83 %); the start and joining of items
 // where there are many short ones (37 sequences of up to 2011 tokens, 12 heads of 64: 24 us, its bytes 8.4); for f32
-// rows the products of two terms each (20 prompts of up to 257 rows, 14 heads over 2 of 64: 120 us, mma.sync pipe 40 %
+// rows the products of two terms each (20 prompts of up to 257 rows, 14 heads over 2 of 64: 127 us, mma.sync pipe 40 %
 // and issue slots 45 % busy at the 8 warps that the registers leave an SM); one sequence of 640 tokens the launch (5.6).
 constexpr uint32_t kWholePages = 128;
 
@@ -327,6 +327,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                         }
                     }
                 }
+                float low[F32 ? NT : 1][4];  // f32 rows: the second terms by themselves (see the other product)
 #pragma unroll
                 for (int w = 0; w < KW; w++) {
                     uint32_t a0, a1, a2, a3;
@@ -337,14 +338,20 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                         if (w == 0)
                             mma_start(u[k][n], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1], qo[n][0], qo[n][1]);
                         else mma_16816(u[k][n], a0, a1, a2, a3, qb[n][0][w][0], qb[n][0][w][1]);
-                        if constexpr (F32) mma_16816(u[k][n], a0, a1, a2, a3, qb[n][F32][w][0], qb[n][F32][w][1]);
+                        if constexpr (F32) {
+                            if (w == 0) mma_start(low[n], a0, a1, a2, a3, qb[n][F32][w][0], qb[n][F32][w][1], 0.f, 0.f);
+                            else mma_16816(low[n], a0, a1, a2, a3, qb[n][F32][w][0], qb[n][F32][w][1]);
+                        }
                     }
                 }
                 // u of tokens tok, tok + 2 and rows 2 t, 2 t + 1
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) u[k][n][e] = fmaf(u[k][n][e], qf[n][e & 1] * pa, pl);
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (F32) u[k][n][e] += low[n][e];
+                        u[k][n][e] = fmaf(u[k][n][e], qf[n][e & 1] * pa, pl);
+                    }
             }
             if (!open) {
 #pragma unroll
@@ -415,7 +422,8 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                     }
                 }
             // f32 rows: the pages' products by themselves, then added to o. The tensor core cuts off what it adds up, and
-            // along contexts of thousands of tokens that grew to 2.0e-6 of an output (now 0.8e-6, for 2 % of the time).
+            // along contexts of thousands of tokens that grew to 2.0e-6 of an output (now, with the second
+            // terms of the scores apart as well, 0.5e-6, for 2 % of the time).
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
                 float z[F32 ? NT : 1][4];
