@@ -20,8 +20,9 @@ struct StepRing {
 // Two f16 from the low (high) two bytes of a word of int8.
 //   EXACT: the whole numbers q themselves.
 //   else:  (q + 128) 2^-24, the byte with its sign bit flipped as a subnormal f16: three instructions a word instead
-//          of five; the products' sums are then off by 128 2^-24 times the sum of the other operand, which the
-//          caller takes off.
+//          of five; a product is then off by 128 2^-24 times the sum of the other operand, which it starts below zero
+//          by. For sums over a head's dims only: along a context the offset grows past what it hides (at 131072 tokens of
+//          diffuse scores an output was 14 % off), so V enters exactly.
 template <bool EXACT>
 __device__ __forceinline__ void bytes_to_f16(uint32_t v, uint32_t& r0, uint32_t& r1) {
     if constexpr (EXACT) {
@@ -64,9 +65,9 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 // The MMA does not care in which order k and the rows of A run, so they run as the page's bytes lie: lane (g, t) takes
 // 16 dims of the tokens 4 (g / 2) + g % 2 (+ 2) for the first product and the four tokens 4 t .. 4 t + 3 of a dim for
 // the second, and P^T is S^T's own fragment, transposed in registers.
-// f32 rows: q and p as two f16 terms each (22 bits), bytes converted exactly. 16-bit rows: q exact, bytes with the
-// offset of bytes_to_f16; p two terms for f16 outputs of up to 8 rows (so that only the output's own rounding
-// remains), one for bf16 and for more rows (2^-11 of p).
+// f32 rows: q and p as two f16 terms each (22 bits), bytes converted exactly. 16-bit rows: q exact, K's bytes with the
+// offset of bytes_to_f16, V's exactly; p two terms for f16 outputs of up to 8 rows (so that only the output's own
+// rounding remains), one for bf16 and for more rows (2^-11 of p).
 //
 // What bounds it: HBM where the contexts are long (64 sequences of 3800 to 4400 tokens, 64 heads over 8 of 128, bf16:
 // 541 MB in 97 us, 85 % of the measured copy rate; the three above 106 us, 83 %); the start and joining of items
@@ -281,16 +282,14 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
             }
         }
 
-        // m: the reference (-inf until a row has seen something); ref: m, or 0; ps: the sum of p as the product sees
-        // it (a product with ones)
-        float o[NT][NJ][4], m[NT][2], ref[NT][2], l[NT][2], ps[NT][4];
+        // m: the reference (-inf until a row has seen something); ref: m, or 0
+        float o[NT][NJ][4], m[NT][2], ref[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
             for (int j = 0; j < NJ; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; e++)
-                m[n][e] = -INFINITY, ref[n][e] = 0.f, l[n][e] = 0.f, ps[n][e] = ps[n][2 + e] = 0.f;
+            for (int e = 0; e < 2; e++) m[n][e] = -INFINITY, ref[n][e] = 0.f, l[n][e] = 0.f;
         }
         const int tok = 4 * (g >> 1) + (g & 1);
         const uint32_t k_at = HD == 32 ? tok * HD + 8 * t : tok * HD + 16 * t, swap = HD == 128 ? (g & 1) << 6 : 0,
@@ -386,7 +385,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                         to = to > m[n][e] + 8.0f ? to : m[n][e];
                         const float f = m[n][e] == -INFINITY ? (to == -INFINITY ? 1.f : 0.f) : ex2(m[n][e] - to);
                         m[n][e] = to, ref[n][e] = to == -INFINITY ? 0.f : to;
-                        l[n][e] *= f, ps[n][e] *= f, ps[n][2 + e] *= f;
+                        l[n][e] *= f;
 #pragma unroll
                         for (int j = 0; j < NJ; j++) o[n][j][e] *= f, o[n][j][2 + e] *= f;
                     }
@@ -408,11 +407,6 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                             pb[k][n][PLO][r] = transpose8(pack_f16(x[2 * r] - z.x, x[2 * r + 1] - z.y));
                         }
                     }
-                    if constexpr (!F32) {
-                        constexpr uint32_t kOne = 0x3c003c00u;
-                        mma_16816(ps[n], kOne, kOne, kOne, kOne, pb[k][n][0][0], pb[k][n][0][1]);
-                        if constexpr (PLO) mma_16816(ps[n], kOne, kOne, kOne, kOne, pb[k][n][PLO][0], pb[k][n][PLO][1]);
-                    }
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         // (p in f32: a page's p may be nothing in f16 next to its part of l. An unseen page's scale may
@@ -421,31 +415,29 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
                         if (open || y != 0.f) l[n][e] = fmaf(y, pi[k], l[n][e]);
                     }
                 }
-            // f32 rows: the pages' products by themselves, then added to o. The tensor core cuts off what it adds up, and
-            // along contexts of thousands of tokens that grew to 2.0e-6 of an output (now, with the second
-            // terms of the scores apart as well, 0.5e-6, for 2 % of the time).
+            // The pages' products by themselves, then added to o: the tensor core cuts off what it adds up, and chained
+            // through, contexts of thousands of tokens were 2.0e-6 off in f32 (now, with the second terms of the scores
+            // apart as well, 0.5e-6).
 #pragma unroll
             for (int j = 0; j < NJ; j++) {
-                float z[F32 ? NT : 1][4];
+                float z[NT][4];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     uint32_t a0, a1, a2, a3;
                     const uint32_t vb = at + k * PB + v_at + 16 * j * kPage;
-                    bytes_to_f16<F32>(lds32(vb), a0, a2);
-                    bytes_to_f16<F32>(lds32(vb + 8 * kPage), a1, a3);
+                    bytes_to_f16<true>(lds32(vb), a0, a2);
+                    bytes_to_f16<true>(lds32(vb + 8 * kPage), a1, a3);
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        float(&d)[4] = F32 ? z[F32 ? n : 0] : o[n][j];
-                        if (F32 && k == 0) mma_start(d, a0, a1, a2, a3, pb[k][n][0][0], pb[k][n][0][1], 0.f, 0.f);
-                        else mma_16816(d, a0, a1, a2, a3, pb[k][n][0][0], pb[k][n][0][1]);
-                        if constexpr (PLO) mma_16816(d, a0, a1, a2, a3, pb[k][n][PLO][0], pb[k][n][PLO][1]);
+                        if (k == 0) mma_start(z[n], a0, a1, a2, a3, pb[k][n][0][0], pb[k][n][0][1], 0.f, 0.f);
+                        else mma_16816(z[n], a0, a1, a2, a3, pb[k][n][0][0], pb[k][n][0][1]);
+                        if constexpr (PLO) mma_16816(z[n], a0, a1, a2, a3, pb[k][n][PLO][0], pb[k][n][PLO][1]);
                     }
                 }
-                if constexpr (F32)
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) o[n][j][e] += z[n][e];
+                    for (int e = 0; e < 4; e++) o[n][j][e] += z[n][e];
             }
             __syncwarp();  // every lane has read the stage
             if (bad) {  // a copy did not come in time: give the ones in flight as long again, and leave
@@ -463,7 +455,6 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
 
         // the warps' parts: (m, l) and o in units of 2^m, through the ring's space
         constexpr int OS = HD + 4;  // floats of a row there (rows 2 t of a warp's stores in distinct banks)
-        float off[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -472,7 +463,6 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
 #pragma unroll
                 for (int k = 4; k < 32; k *= 2) y += __shfl_xor_sync(0xffffffffu, y, k);
                 if (g == 0) ml[warp][0][8 * n + 2 * t + e] = m[n][e], ml[warp][1][8 * n + 2 * t + e] = y;
-                off[n][e] = -128.0f * ps[n][e];
             }
         __syncthreads();
         float* os = reinterpret_cast<float*>(smem);  // [warp][RT][OS]
@@ -482,8 +472,7 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
             for (int j = 0; j < NJ; j++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    os[((size_t)warp * RT + 8 * n + 2 * t + (e & 1)) * OS + 16 * j + 8 * (e >> 1) + g] =
-                        F32 ? o[n][j][e] : fmaf(o[n][j][e], 16777216.0f, off[n][e & 1]);
+                    os[((size_t)warp * RT + 8 * n + 2 * t + (e & 1)) * OS + 16 * j + 8 * (e >> 1) + g] = o[n][j][e];
         __syncthreads();
         float* part = p.part + (size_t)(2 * blockIdx.x + (blockIdx.x == c0)) * RT * (HD + 2);
         const int valid = min(RT, rows - row0);
