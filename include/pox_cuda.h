@@ -398,7 +398,8 @@ typedef struct {
 /* Appends k and v (rows [batch->rows][kv_heads], one dtype; k rotated on the way unless rope is NULL or
  * has rot_dim 0) at their positions. Scale rule, per page, kv head and side, in f32:
  *   s' = max(s, max |x| / 127) over the rows that go to the page, s = 0 when slot 0 is among them;
- *   a new element is stored as rint(x / s'), an element of an older slot as rint(byte * (s / s')).
+ *   a new element is stored as rint(x / s') (at most 127 in magnitude, where a subnormal s' is coarser
+ *   than that), an element of an older slot as rint(byte * (s / s')).
  * Older slots are the ones below the page's first new row; a page's scale never falls until its slot 0 is
  * written again. Elements that are not finite do not enter the maximum: an infinity is stored as
  * +-127, a NaN as 0. Two rows at one position in one call are not allowed. */

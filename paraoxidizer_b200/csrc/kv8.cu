@@ -410,12 +410,13 @@ __global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uin
         m = joined(m);
         const float now = fmaxf(old, __fdiv_rn(m, 127.f));
         up = now < 0x1p-64f ? 0x1p64f : now > 0x1p64f ? 0x1p-64f : 1.f;
+        const float most = 127.f * (now * up);  // (a subnormal scale is coarse: up to 190 such steps in an element)
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const float y = v[t][e];
-                v[t][e] = y != y ? 0.f : fabsf(y) < INFINITY ? y * up : copysignf(127.f * (now * up), y);
+                v[t][e] = y != y ? 0.f : fminf(fmaxf(y * up, -most), most);
             }
     }
     if (!live) return;

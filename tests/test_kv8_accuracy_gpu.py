@@ -1,11 +1,11 @@
 """How far attention over the 8-bit cache may be off in norm, against the outputs' own size.
 
-Queries and values are independent normal values, so an output is a random walk over its context: sum p_t v_t of
-n tokens is sqrt(n) smaller than the sum of magnitudes, and an error that keeps to a token's own size does not hide in it.
+Queries and values are independent normal values, so an output is a random walk over its context: sum p_t v_t of n
+tokens is sqrt(n) smaller than the sum of magnitudes, and an error of a token's own size does not hide in it.
 Bounds are of the norm over all outputs, relative to the norm of the outputs:
   * rounding to the rows' type: measured on the 64-bit result itself;
-  * p rounded to 11 bits (16-bit rows other than f16 with at most 8 rows of a kv head): each p is off by at most 2^-11 of
-    itself, 2^-11 / sqrt(3) in the root mean square at most, independently of v, so that the walk is off by as much;
+  * p rounded to 11 bits (16-bit rows other than f16 with at most 8 rows of a kv head): each p is off by at most 2^-11
+    of itself, 2^-11 / sqrt(3) in the root mean square at most, independently of v, so that the walk is off by as much;
   * f32 arithmetic: a score u = s + log2 b of 8 to 16 is rounded to 2^-20 / sqrt(12) = 2.8e-7 (root mean square, times
     ln 2), its products carry about 2e-7, the exponential 2^-22.5, sums of the pages' products at most 1024 roundings
     to nearest of 2^-24 / sqrt(3) each (1.1e-6 at 131072 tokens of one warp set). Together below 1.3e-6; the bound is
@@ -44,7 +44,8 @@ class Shared:
         g = torch.Generator(device="cuda").manual_seed(seed)
         nb = (ctx + PAGE - 1) // PAGE
         self.hd, self.ctx, self.group, self.rows = hd, ctx, heads // kvh, rows
-        self.pages = (torch.randn(nb, kvh, 32 * hd, generator=g, device="cuda") * 36).round().clamp(-127, 127).to(torch.int8)
+        x = torch.randn(nb, kvh, 32 * hd, generator=g, device="cuda") * 36
+        self.pages = x.round().clamp(-127, 127).to(torch.int8)
         self.scales = (torch.rand(nb, kvh, 2, generator=g, device="cuda") * 0.6).exp() * 0.02
         self.tab = torch.randperm(nb, generator=g, device="cuda").int()[None].repeat(seqs, 1).contiguous()
         self.starts = torch.arange(seqs + 1, device="cuda", dtype=torch.int32) * rows
@@ -52,8 +53,8 @@ class Shared:
         self.q = torch.randn(seqs * rows, heads, hd, generator=g, device="cuda").to(dt)
         self.out = torch.empty_like(self.q)
         self.cache = L.Kv8Cache(self.pages.data_ptr(), self.scales.data_ptr(), nb, kvh, hd)
-        self.batch = L.Kv8Batch(self.starts.data_ptr(), self.lens.data_ptr(), self.tab.data_ptr(), seqs, seqs * rows, rows,
-                                ctx, nb)
+        self.batch = L.Kv8Batch(self.starts.data_ptr(), self.lens.data_ptr(), self.tab.data_ptr(), seqs, seqs * rows,
+                                rows, ctx, nb)
         self.view = lambda t: L.Rows(t.data_ptr(), code, t.stride(0), t.stride(1))
 
     def attend(self, be):
@@ -90,7 +91,7 @@ def off(x, ref):
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("seqs,rows,ctx,heads,kvh,hd", [
-    (600, 1, 20001, 1, 1, 64),      # more sequences than CTAs: none is split, a warp goes through a quarter of a context
+    (600, 1, 20001, 1, 1, 64),      # more sequences than CTAs: a warp goes through a quarter of a context
     (600, 1, 131072, 1, 1, 64),
     (450, 1, 16380, 8, 1, 128),
     (300, 2, 8190, 6, 1, 32),       # 12 rows of a kv head

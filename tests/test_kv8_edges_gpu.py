@@ -1,0 +1,75 @@
+"""The 8-bit paged KV cache where its calls can go wrong: magnitudes at the ends of f32.
+
+Stored bytes and scales follow the rule element by element in f32, so they are compared for equality with its numpy
+restatement (test_kv8_gpu.np_append)."""
+import numpy as np
+import pytest
+from test_kv8_gpu import STREAM, Cache, np_append, rows_of
+
+from paraoxidizer_b200 import _lib as L
+from paraoxidizer_b200.backend import CudaBackend
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def be():
+    b = CudaBackend.create(0)
+    yield b
+    b.synchronize()
+    b.close()
+
+
+def check_append(be, c, starts, ctx, k, v):
+    pages, scales = c.pages.cpu().numpy(), c.scales.cpu().numpy()
+    with np.errstate(all="ignore"):
+        np_append(pages, scales, c, c.tab_np, starts, ctx, k.float().cpu().numpy(), v.float().cpu().numpy(), None, 0,
+                  False)
+    be.kv8_append(c.c, c.batch(starts, ctx), rows_of(k), rows_of(v), None, STREAM)
+    be.synchronize()
+    assert np.array_equal(c.scales.cpu().numpy(), scales, equal_nan=True)
+    used = [b for s, x in enumerate(ctx) for b in c.tab_np[s, :(x + 15) // 16]]
+    assert np.array_equal(c.pages.cpu().numpy()[used], pages[used])
+
+
+# largest magnitudes of a page, in units of 2^-149: around the steps of the rounded scale m / 127
+SMALL = [1, 63, 64, 100, 127, 128, 150, 189, 190, 191, 254, 317, 318, 1000, 16129, 16192, 2 ** 22, 2 ** 23 - 1, 2 ** 23]
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("most", SMALL)
+def test_append_of_subnormal_magnitudes(be, hd, most):
+    rng = np.random.default_rng(most)
+    n = 21
+    units = rng.integers(-most, most + 1, size=(2, n, 2, hd))
+    units[:, ::5, :, 3], units[:, 1::5, :, hd - 1] = most, -most
+    sign = (units < 0).astype(np.uint32) << np.uint32(31)
+    x = (np.abs(units).astype(np.uint32) | sign).view(np.float32)
+    k, v = (torch.from_numpy(a.copy()).cuda() for a in x)
+    c = Cache([n], 2, hd, fill=False)
+    check_append(be, c, [0, 17], [17], k[:17].contiguous(), v[:17].contiguous())
+    check_append(be, c, [0, 4], [21], k[17:].contiguous(), v[17:].contiguous())  # onto older slots of such a page
+
+
+@pytest.mark.parametrize("size", [2.0 ** -126, 2.0 ** -100, 2.0 ** -91, 2.0 ** -90, 2.0 ** -64, 2.0 ** -57, 2.0 ** 57,
+                                  2.0 ** 71, 2.0 ** 119, 2.0 ** 120, 2.0 ** 125])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_append_where_a_scale_s_reciprocal_leaves_the_range(be, dtype, size):
+    dt = torch.float32 if dtype == "f32" else torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(40, 3, 64, generator=g, device="cuda").clamp(-5, 5).mul(size).to(dt) for _ in range(2))
+    v[7, 1, 2], v[9, 0, 0], v[11, 2, 63] = float("inf"), float("-inf"), float("nan")
+    c = Cache([40], 3, 64, fill=False)
+    check_append(be, c, [0, 21], [21], k[:21], v[:21])
+    check_append(be, c, [0, 1], [22], k[21:22] * 2, v[21:22] * 0.5)  # the older slots of one side follow
+    check_append(be, c, [0, 18], [40], k[22:], v[22:])
+
+
+def test_append_of_small_rows_onto_large_pages_and_back(be):
+    """A page whose scale is huge takes rows of nothing, and the other way round."""
+    c = Cache([16], 1, 64, fill=False)
+    one = torch.ones(1, 1, 64, device="cuda")
+    for i, power in enumerate([-149, -140, -120, -60, 0, 60, 126, -149]):
+        x = one * 2.0 ** power * 1.25
+        check_append(be, c, [0, 1], [i + 1], x, -x)
