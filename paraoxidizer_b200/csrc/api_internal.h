@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <mutex>
+#include <thread>
 #include <unordered_map>
 #include <vector>
 
@@ -45,9 +46,17 @@ struct pox_tensor {
 namespace pox {
 // What the attention over the 8-bit cache keeps for each stream that calls it (calls on different
 // streams may overlap): the parts of items that are cut, and their tickets, zero between launches.
+// A stream is known by its id: a handle is given out again after its stream, whose last work may
+// still run, and cudaStreamPerThread is one handle for a stream of each thread.
 struct Kv8Scratch {
     float* part = nullptr;
-    uint32_t* tickets = nullptr;  // behind the parts, once they are cleared
+    uint32_t* tickets = nullptr;   // behind the parts, once they are cleared
+    cudaStream_t handle = nullptr;
+    std::thread::id thread;        // of the first call: cudaStreamPerThread is another stream in another thread
+    bool captured = false;         // a graph holds the addresses
+    bool over = false;             // the handle came back under another id: the stream is destroyed
+    bool idle = false;             // .. and its work is done: another stream may take the place
+    uint64_t over_since = 0;       // pox_cuda_ctx::syncs then
 };
 }  // namespace pox
 
@@ -77,7 +86,8 @@ struct pox_cuda_ctx {
     size_t tc_tickets_n = 0;
     void* attn_scratch = nullptr;  // kernel-level paged attention: split partials
     size_t attn_scratch_bytes = 0;
-    std::unordered_map<cudaStream_t, pox::Kv8Scratch> kv8;
+    std::unordered_map<unsigned long long, pox::Kv8Scratch> kv8;  // by stream id
+    uint64_t syncs = 0;  // calls of pox_cuda_synchronize so far
     int* err_host = nullptr;  // kernel error flag (host-mapped); nonzero = a bounded wait expired or bad input
     int* err_dev = nullptr;
     std::vector<pox_model*> models;  // decode models created on this context (destroyed with it)

@@ -626,28 +626,64 @@ static bool prompt_is_faster(const pox_kv8_cache* c, const pox_kv8_batch* b, int
 }
 
 // The stream's places for the parts of items that a plan cuts, and their tickets: made by its first call, as large as any
-// plan on this device asks for, and kept as long as the context (a captured graph holds their addresses).
+// plan on this device asks for, and not moved (a captured graph holds their addresses). Those of a stream that is
+// known to be destroyed go to the next new one, after a pox_cuda_synchronize and unless they were captured.
 static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, Kv8StepPlan& p) {
     try {
         std::lock_guard<std::mutex> lk(ctx->mu);
-        Kv8Scratch& k = ctx->kv8[st];
-        if (!k.tickets) {
-            cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-            if (cudaStreamIsCapturing(st, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone)
-                return set_error(POX_ERR_INVALID, "the parts' places must be allocated by a call before stream capture");
+        auto same_handle = [&](const Kv8Scratch& x) {
+            return x.handle == st && (st != cudaStreamPerThread || x.thread == std::this_thread::get_id()) && !x.over;
+        };
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        cudaError_t e = cudaStreamIsCapturing(st, &cs);
+        if (e != cudaSuccess) return cuda_error(e, "stream of kv8_attention");
+        if (cs != cudaStreamCaptureStatusNone) {  // (a stream's id is not to be had while it is captured)
+            for (auto& k : ctx->kv8)
+                if (same_handle(k.second) && k.second.tickets) {
+                    k.second.captured = true;
+                    p.part = k.second.part, p.tickets = k.second.tickets;
+                    return POX_OK;
+                }
+            return set_error(POX_ERR_INVALID, "the parts' places must be allocated by a call before stream capture");
+        }
+        unsigned long long id = 0;
+        e = cudaStreamGetId(st, &id);
+        if (e != cudaSuccess) return cuda_error(e, "stream of kv8_attention");
+        auto at = ctx->kv8.find(id);
+        if (at == ctx->kv8.end() || !at->second.tickets) {
+            if (at == ctx->kv8.end()) {
+                auto idle = ctx->kv8.end();
+                for (auto k = ctx->kv8.begin(); k != ctx->kv8.end(); ++k) {
+                    if (same_handle(k->second)) k->second.over = true, k->second.over_since = ctx->syncs;
+                    if (k->second.idle) idle = k;
+                }
+                if (idle == ctx->kv8.end()) {
+                    at = ctx->kv8.emplace(id, Kv8Scratch()).first;
+                } else {
+                    float* part = idle->second.part;
+                    auto node = ctx->kv8.extract(idle);
+                    node.key() = id;
+                    node.mapped() = Kv8Scratch();
+                    node.mapped().part = part;
+                    at = ctx->kv8.insert(std::move(node)).position;
+                }
+                at->second.handle = st;
+                at->second.thread = std::this_thread::get_id();
+            }
+            Kv8Scratch& k = at->second;
             const size_t tickets = (size_t)Kv8StepPlan::most_ctas(ctx->num_sms) * sizeof(uint32_t);
             if (!k.part) {
-                const cudaError_t e = cudaMalloc(&k.part, Kv8StepPlan::most_part_bytes(ctx->num_sms) + tickets);
+                e = cudaMalloc(&k.part, Kv8StepPlan::most_part_bytes(ctx->num_sms) + tickets);
                 if (e != cudaSuccess) return cuda_error(e, "split partials");
             }
-            uint32_t* at = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(k.part) +
-                                                       Kv8StepPlan::most_part_bytes(ctx->num_sms));
-            const cudaError_t e = cudaMemsetAsync(at, 0, tickets, st);
+            uint32_t* t = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(k.part) +
+                                                      Kv8StepPlan::most_part_bytes(ctx->num_sms));
+            e = cudaMemsetAsync(t, 0, tickets, st);
             if (e != cudaSuccess) return cuda_error(e, "split partials");
-            k.tickets = at;
+            k.tickets = t;
         }
-        p.part = k.part;
-        p.tickets = k.tickets;
+        p.part = at->second.part;
+        p.tickets = at->second.tickets;
     } catch (const std::exception& x) {  // (no exception crosses the C boundary)
         return set_error(POX_ERR_OOM, "split partials: %s", x.what());
     }

@@ -167,7 +167,16 @@ int pox::take_kernel_error(pox_cuda_ctx* ctx) {
 extern "C" int pox_cuda_synchronize(pox_cuda_ctx* ctx) {
     if (!ctx) return set_error(POX_ERR_INVALID, "ctx is NULL");
     CK(cudaSetDevice(ctx->device), "cudaSetDevice");
+    uint64_t n;
+    {
+        std::lock_guard<std::mutex> lk(ctx->mu);
+        n = ++ctx->syncs;
+    }
     CK(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+    {
+        std::lock_guard<std::mutex> lk(ctx->mu);
+        for (auto& k : ctx->kv8) k.second.idle |= k.second.over && !k.second.captured && k.second.over_since < n;
+    }
     return take_kernel_error(ctx);
 }
 

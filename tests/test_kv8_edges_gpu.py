@@ -1,7 +1,11 @@
-"""The 8-bit paged KV cache where its calls can go wrong: magnitudes at the ends of f32.
+"""The 8-bit paged KV cache where its calls can go wrong: magnitudes at the ends of f32, streams that share a
+handle.
 
 Stored bytes and scales follow the rule element by element in f32, so they are compared for equality with its numpy
 restatement (test_kv8_gpu.np_append)."""
+import ctypes
+import threading
+
 import numpy as np
 import pytest
 from test_kv8_gpu import STREAM, Cache, np_append, rows_of
@@ -73,3 +77,72 @@ def test_append_of_small_rows_onto_large_pages_and_back(be):
     for i, power in enumerate([-149, -140, -120, -60, 0, 60, 126, -149]):
         x = one * 2.0 ** power * 1.25
         check_append(be, c, [0, 1], [i + 1], x, -x)
+
+
+class Steps:
+    """Single tokens over long contexts, which the GPU splits and joins through the stream's partials."""
+
+    def __init__(self, seed, ctx):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.c = Cache(ctx, 2, 64, seed=seed)
+        self.b = self.c.batch(list(range(len(ctx) + 1)), ctx)
+        self.q = torch.randn(len(ctx), 8, 64, generator=g, device="cuda")
+
+    def attend(self, be, out, stream):
+        be.kv8_attention(self.c.c, self.b, rows_of(self.q), rows_of(out), 8, 0.0, stream)
+
+
+def test_threads_on_the_per_thread_stream_have_partials_of_their_own(be):
+    per_thread = 2  # cudaStreamPerThread: one handle, a stream of each thread
+    work = [Steps(1, [30001, 9000]), Steps(2, [12345, 4567, 20000])]
+    want = [torch.empty_like(w.q) for w in work]
+    outs = [[torch.empty_like(w.q) for _ in range(200)] for w in work]
+    for w, o in zip(work, want):
+        w.attend(be, o, STREAM)
+    be.synchronize()
+    errors, gate = [], threading.Barrier(2)
+
+    def run(i):
+        try:
+            gate.wait()
+            for o in outs[i]:
+                work[i].attend(be, o, per_thread)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    be.synchronize()
+    assert not errors
+    for o, w in zip(outs, want):
+        assert all(torch.equal(x, w) for x in o)
+
+
+def test_streams_that_come_and_go(be):
+    """Streams created and destroyed while their work runs (the driver gives handles out again): right results, and partials
+    that are taken over instead of piling up."""
+    cuda = ctypes.CDLL("libcuda.so.1")
+    w = Steps(3, [50000, 31000])
+    want = torch.empty_like(w.q)
+    w.attend(be, want, STREAM)
+    be.synchronize()
+    handles, free = set(), None
+    for i in range(12):
+        outs = [torch.empty_like(w.q) for _ in range(8)]
+        torch.cuda.synchronize()
+        for o in outs:
+            s = ctypes.c_void_p()
+            assert cuda.cuStreamCreate(ctypes.byref(s), 1) == 0
+            w.attend(be, o, s.value)
+            w.attend(be, o, s.value)
+            assert cuda.cuStreamDestroy_v2(s) == 0
+            handles.add(s.value)
+        be.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+        if i == 5:
+            free = torch.cuda.mem_get_info()[0]
+    if len(handles) < 48:  # handles did come back
+        assert torch.cuda.mem_get_info()[0] > free - 64 * 2 ** 20
