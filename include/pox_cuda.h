@@ -386,8 +386,9 @@ typedef struct {
  * block_tables[s * max_blocks_per_seq + position / 16]. A row whose position is negative is padding (a
  * free slot of a fixed batch: ctx_lens[s] = 0). max_rows and max_ctx bound the rows and the context of
  * any sequence (max_ctx <= 16 max_blocks_per_seq); they choose the launch. A sequence that breaks a
- * bound, and pages outside [0, num_blocks), are left out on the device and the next
- * pox_cuda_synchronize returns POX_ERR_INVALID. */
+ * bound or whose row starts are not as said (the first one's begins at 0, the last one's ends at `rows`),
+ * and pages outside [0, num_blocks), are left out on the device and the next pox_cuda_synchronize returns
+ * POX_ERR_INVALID. */
 typedef struct {
     const uint32_t* row_starts;
     const uint32_t* ctx_lens;

@@ -230,12 +230,7 @@ __device__ __forceinline__ bool page_unit(const Kv8Batch& b, uint32_t item, Page
     o.first = kPage, o.last = 0, o.page = 0, o.row = 0, o.blk = 0, o.bytes = nullptr;
     if (!seq_span(b, s, o.sp, err)) return false;
     const int begin = o.sp.ctx - o.sp.n, p0 = max(begin, 0);
-    const int j = (int)(item - page_base(b, s));
-    if (j < 0) {  // row_starts does not begin at 0
-        atomicOr(err, kErrBatch);
-        return false;
-    }
-    o.page = p0 / kPage + j;
+    o.page = p0 / kPage + (int)(item - page_base(b, s));
     if (o.sp.ctx <= p0 || o.page * kPage >= o.sp.ctx) return true;
     o.first = max(p0 - o.page * kPage, 0), o.last = min(o.sp.ctx - o.page * kPage, kPage);
     o.row = (size_t)o.sp.r0 + (o.page * kPage + o.first - begin);
@@ -604,8 +599,9 @@ static Kv8Cache cache_view(const pox_kv8_cache* c) {
 static Kv8Batch batch_view(const pox_kv8_batch* b) {
     // as many rows as sequences and at most one each: one each, and no search on the device
     const bool single = b->max_rows == 1 && b->rows == b->seqs;
-    return Kv8Batch{single ? nullptr : b->row_starts,   b->ctx_lens, b->block_tables,       b->seqs, b->rows,
-                    std::min(b->max_rows, b->rows), b->max_ctx,  b->max_blocks_per_seq};
+    return Kv8Batch{single ? nullptr : b->row_starts, b->ctx_lens, b->block_tables,       b->seqs, b->rows,
+                    std::min(b->max_rows, b->rows),   b->max_ctx,  b->max_blocks_per_seq,
+                    single ? b->row_starts : nullptr};
 }
 
 constexpr int kPromptRows = 64;

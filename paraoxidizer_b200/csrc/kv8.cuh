@@ -36,6 +36,7 @@ struct Kv8Batch {
     const uint32_t* ctx_lens;
     const int32_t* btab;
     uint32_t seqs, rows, max_rows, max_ctx, mbps;
+    const uint32_t* ones;  // row_starts as given where they have to be 0, 1, 2, .. (row_starts is then NULL)
 };
 
 template <typename T>
@@ -77,16 +78,20 @@ __device__ __forceinline__ float2 rope_turn(float a, float b, float2 cs) {
                        __fadd_rn(__fmul_rn(a, cs.y), __fmul_rn(b, cs.x)));
 }
 
-// Rows, context and first row of sequence s; false (reported) if it breaks the batch's bounds.
+// Rows, context and first row of sequence s; false (reported) if it breaks the batch's bounds or its row starts do not
+// fit: they begin at 0, end at the batch's rows and, in a batch of one row each, count up.
 struct SeqSpan {
     uint32_t r0;
     int n, ctx;
 };
 __device__ __forceinline__ bool seq_span(const Kv8Batch& b, uint32_t s, SeqSpan& o, int* err) {
-    const uint32_t r0 = b.row_starts ? b.row_starts[s] : s, r1 = b.row_starts ? b.row_starts[s + 1] : s + 1;
-    const uint32_t ctx = b.ctx_lens[s];
+    const uint32_t* starts = b.row_starts ? b.row_starts : b.ones;
+    const uint32_t r0 = starts ? starts[s] : s, r1 = starts ? starts[s + 1] : s + 1, ctx = b.ctx_lens[s];
     o.r0 = r0, o.n = (int)(r1 - r0), o.ctx = (int)ctx;
-    if (r1 < r0 || r1 > b.rows || r1 - r0 > b.max_rows || ctx > b.max_ctx) {
+    const bool fits = b.row_starts ? (s || !r0) && (s + 1 < b.seqs || r1 == b.rows) && r1 >= r0 && r1 <= b.rows &&
+                                         r1 - r0 <= b.max_rows
+                                   : r0 == s && r1 == s + 1;
+    if (!fits || ctx > b.max_ctx) {
         atomicOr(err, kErrBatch);
         return false;
     }

@@ -1,5 +1,5 @@
 """The 8-bit paged KV cache where its calls can go wrong: magnitudes at the ends of f32, streams that share a
-handle.
+handle, row starts that do not describe the rows.
 
 Stored bytes and scales follow the rule element by element in f32, so they are compared for equality with its numpy
 restatement (test_kv8_gpu.np_append)."""
@@ -122,8 +122,8 @@ def test_threads_on_the_per_thread_stream_have_partials_of_their_own(be):
 
 
 def test_streams_that_come_and_go(be):
-    """Streams created and destroyed while their work runs (the driver gives handles out again): right results, and partials
-    that are taken over instead of piling up."""
+    """Streams created and destroyed while their work runs (the driver gives handles out again): right results, and
+    partials that are taken over instead of piling up."""
     cuda = ctypes.CDLL("libcuda.so.1")
     w = Steps(3, [50000, 31000])
     want = torch.empty_like(w.q)
@@ -146,3 +146,58 @@ def test_streams_that_come_and_go(be):
             free = torch.cuda.mem_get_info()[0]
     if len(handles) < 48:  # handles did come back
         assert torch.cuda.mem_get_info()[0] > free - 64 * 2 ** 20
+
+
+# row starts, rows, the bound of a sequence's rows, sequences left out
+STARTS = [
+    ([0, 2, 2], 2, 1, [0, 1]),       # as many rows as sequences, at most one each, but not one each
+    ([1, 1, 2], 2, 1, [0]),
+    ([0, 1, 2, 2], 3, 1, [2]),       # the third row belongs to no sequence
+    ([3, 6, 9], 9, 3, [0]),          # the first rows belong to none
+    ([20, 60, 90], 90, 60, [0]),
+    ([0, 3, 7], 9, 4, [1]),          # nor the last
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("starts,rows,most,out_of", STARTS)
+def test_row_starts_that_do_not_fit_are_reported_and_left_out(be, dtype, starts, rows, most, out_of):
+    dt = torch.float32 if dtype == "f32" else torch.bfloat16
+    seqs = len(starts) - 1
+    ctx = [50 + 40 * s + most for s in range(seqs)]
+    c = Cache(ctx, 2, 64, seed=rows)
+    b = c.batch(starts, ctx)
+    b.row_starts, b.rows, b.max_rows = c.keep[0].data_ptr(), rows, most
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(rows, h, 64, generator=g, device="cuda").to(dt) for h in (4, 2, 2))
+    out, ko, vo = (torch.full_like(t, 7.0) for t in (q, k, v))
+    kept = [s for s in range(seqs) if s not in out_of]
+    own = torch.zeros(rows, dtype=torch.bool)
+    for s in kept:
+        own[starts[s]:starts[s + 1]] = True
+    before = c.pages.clone(), c.scales.clone()
+    for call in (lambda: be.kv8_attention(c.c, b, rows_of(q), rows_of(out), 4, 0.0, STREAM),
+                 lambda: be.kv8_read(c.c, b, rows_of(ko), rows_of(vo), STREAM),
+                 lambda: be.kv8_append(c.c, b, rows_of(k), rows_of(v), None, STREAM)):
+        call()
+        with pytest.raises(L.PoxError, match="bounds"):
+            be.synchronize()
+    for t in (out, ko, vo):
+        assert bool((t[~own] == 7.0).all()) and not bool((t[own] == 7.0).all(-1).any())
+    for s in range(seqs):
+        blocks = torch.from_numpy(c.tab_np[s, :(ctx[s] + 15) // 16].astype(np.int64)).cuda()
+        same = torch.equal(c.pages[blocks], before[0][blocks]) and torch.equal(c.scales[blocks], before[1][blocks])
+        assert same == (s in out_of)
+
+
+@pytest.mark.parametrize("rows,starts", [(3000, [100, 3000]), (3000, [0, 2900])])
+def test_row_starts_of_a_prompt_that_do_not_fit(be, rows, starts):
+    c = Cache([3000], 8, 128, seed=1)
+    b = c.batch(starts, [3000])
+    b.row_starts, b.rows, b.max_rows = c.keep[0].data_ptr(), rows, rows
+    q = torch.randn(rows, 32, 128, device="cuda").half()
+    out = torch.full_like(q, 7.0)
+    be.kv8_attention(c.c, b, rows_of(q), rows_of(out), 32, 0.0, STREAM)
+    with pytest.raises(L.PoxError, match="bounds"):
+        be.synchronize()
+    assert bool((out == 7.0).all())
