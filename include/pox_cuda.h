@@ -403,7 +403,9 @@ typedef struct {
  *   than that), an element of an older slot as rint(byte * (s / s')).
  * Older slots are the ones below the page's first new row; a page's scale never falls until its slot 0 is
  * written again. Elements that are not finite do not enter the maximum: an infinity is stored as
- * +-127, a NaN as 0. Two rows at one position in one call are not allowed. */
+ * +-127, a NaN as 0. Two rows at one position in one call are not allowed. A page that a row at a position
+ * outside the rotation table goes to stays as it was, k and v, and the next pox_cuda_synchronize returns
+ * POX_ERR_INVALID; the batch's other pages are written. */
 int pox_cuda_kv8_append(pox_cuda_ctx* ctx, const pox_kv8_cache* cache, const pox_kv8_batch* batch, const pox_rows* k,
                         const pox_rows* v, const pox_rope* rope, void* stream);
 /* Reads rows back: k and v (both rows [batch->rows][kv_heads], one dtype) receive byte * scale of the

@@ -296,7 +296,8 @@ __global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uin
     PageUnit o;
     bool live = page_unit(a.b, item, o, a.err) && u < 2 * a.c.kvh && o.first < o.last;
     const int rot = TURN == kTurnNone || side ? 0 : a.rope.rot, half = rot / 2, pos0 = o.page * kPage + t0;
-    if (live && rot && (uint32_t)(o.page * kPage + o.last - 1) >= a.rope.positions) {
+    // a page with a row outside the table stays as it is, v too
+    if (live && TURN != kTurnNone && a.rope.rot && (uint32_t)(o.page * kPage + o.last - 1) >= a.rope.positions) {
         if (c == 0) atomicOr(a.err, kErrRopePos);
         live = false;
     }

@@ -1,5 +1,6 @@
 """The 8-bit paged KV cache where its calls can go wrong: magnitudes at the ends of f32, streams that share a
-handle, row starts that do not describe the rows.
+handle, row starts that do not describe the rows,
+positions outside the rotation table.
 
 Stored bytes and scales follow the rule element by element in f32, so they are compared for equality with its numpy
 restatement (test_kv8_gpu.np_append)."""
@@ -8,7 +9,7 @@ import threading
 
 import numpy as np
 import pytest
-from test_kv8_gpu import STREAM, Cache, np_append, rows_of
+from test_kv8_gpu import STREAM, Cache, np_append, rope_table, rows_of
 
 from paraoxidizer_b200 import _lib as L
 from paraoxidizer_b200.backend import CudaBackend
@@ -201,3 +202,29 @@ def test_row_starts_of_a_prompt_that_do_not_fit(be, rows, starts):
     with pytest.raises(L.PoxError, match="bounds"):
         be.synchronize()
     assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype,rot,half,pad", [("bf16", 64, True, 0), ("f32", 64, False, 0), ("f16", 6, True, 0),
+                                                ("f32", 64, True, 1)])
+def test_append_outside_the_rotation_table_leaves_the_page(be, dtype, rot, half, pad):
+    """Pages of slots 0 and later, and one that holds older tokens; `pad` takes the rows off the vector loads."""
+    dt = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    ctx, starts, positions = [50, 20, 40], [0, 40, 43, 47], 36
+    c = Cache(ctx, 2, 64, seed=5)
+    table = rope_table(positions, rot)
+    rope = L.Rope(table.data_ptr(), positions, rot, L.POX_ROPE_HALF if half else L.POX_ROPE_INTERLEAVED)
+    k, v = (torch.randn(47, 2, 64 + pad, device="cuda").mul(9).to(dt)[..., :64] for _ in range(2))
+    before, scales = c.pages.clone(), c.scales.clone()
+    be.kv8_append(c.c, c.batch(starts, ctx), rows_of(k), rows_of(v), rope, STREAM)
+    with pytest.raises(L.PoxError, match="rotation table"):
+        be.synchronize()
+    # sequence 0 takes tokens 10 .. 49, 1 takes 17 .. 19, 2 takes 36 .. 39: pages whose last new row is past 35 stay
+    changed = {(0, 0), (0, 1), (1, 1)}
+    for s, x in enumerate(ctx):
+        for page in range((x + 15) // 16):
+            b = c.tab_np[s, page]
+            for side in range(2):
+                same = torch.equal(c.scales[b, :, side], scales[b, :, side])
+                half_page = slice(16 * 64 * side, 16 * 64 * (side + 1))
+                same = same and torch.equal(c.pages[b, :, half_page], before[b, :, half_page])
+                assert same == ((s, page) not in changed), (s, page, side)
