@@ -10,6 +10,10 @@ Bounds are of the norm over all outputs, relative to the norm of the outputs:
     ln 2), its products carry about 2e-7, the exponential 2^-22.5, sums of the pages' products at most 1024 roundings
     to nearest of 2^-24 / sqrt(3) each (1.1e-6 at 131072 tokens of one warp set). Together below 1.3e-6; the bound is
     2^-18.
+  * f32 rows over ordinary contexts (unit normal queries, scores of about 1): the rounding of u, then of 4 to 8, is
+    1e-7, the second terms of q leave 2^-23 / sqrt(3) of a score, the tensor core cuts off 2^-24 of it on average in
+    each of at most 8 steps (3e-7 if all of them point the same way), the exponential 2^-22.5 / sqrt(3). Together
+    0.4e-6; the bound is 1.2e-6. Products without the second terms are off by 2^-12: the last test makes sure of it.
 These add up as squares (they are independent); 1 % is left for their random correlation.
 """
 import math
@@ -104,3 +108,14 @@ def test_long_contexts_keep_the_accuracy_of_short_ones(be, dtype, seqs, rows, ct
     few = rows * heads // kvh <= 8
     p = 0.0 if dtype == "f32" or dtype == "f16" and few else 2.0 ** -11 / math.sqrt(3)
     assert off(got, ref) <= 1.01 * math.sqrt(own ** 2 + p ** 2 + 2.0 ** -36)
+
+
+@pytest.mark.parametrize("seqs,rows,ctx,heads,kvh,hd", [
+    (9, 1, 31, 8, 2, 128), (9, 1, 64, 4, 4, 64), (5, 1, 640, 32, 8, 128), (3, 1, 2500, 14, 2, 64),
+    (40, 1, 5000, 8, 1, 128), (1, 1, 9000, 8, 8, 32), (3, 20, 700, 8, 2, 128), (2, 130, 3000, 14, 2, 64), (1, 513, 4000, 4, 1, 128)])
+def test_f32_rows_carry_f32(be, seqs, rows, ctx, heads, kvh, hd):
+    s = Shared(seqs, rows, ctx, heads, kvh, hd, "f32")
+    ref = s.formula()
+    assert off(s.attend(be), ref) <= 1.2e-6
+    for half in (dict(q_term=lambda x: x.half()), dict(p_term=lambda x: x.half())):
+        assert off(s.formula(**half), ref) > 1e-5
