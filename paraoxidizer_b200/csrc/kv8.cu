@@ -705,16 +705,18 @@ static cudaError_t launch_qk(pox_cuda_ctx* ctx, const pox_qk_norm_rope* a, cudaS
             vec = vec && (((uintptr_t)k.in[i].data | (uintptr_t)k.out[i].data | (uintptr_t)k.w[i]) & 15) == 0 &&
                   ((k.in[i].row | k.in[i].head | k.out[i].row | k.out[i].head) % V) == 0;
     if (!vec) {
-        const unsigned long long items = (unsigned long long)a->rows * nh;
-        return launch_pdl(qk_norm_rope_any_kernel<T>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, st, k);
+        const unsigned long long grid = ((unsigned long long)a->rows * nh + 7) / 8;
+        if (grid > 0x7fffffffu) return cudaErrorInvalidConfiguration;
+        return launch_pdl(qk_norm_rope_any_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, k);
     }
     // as many groups of heads to a warp as leave every SM its 32 warps
     const int all = (nh * L + 31) / 32;
     const int steps = (int)std::min<long long>(std::max<long long>((long long)a->rows * all / (32LL * ctx->num_sms), 1),
                                                std::min(all, 10));
     const int groups = (all + steps - 1) / steps;
-    const unsigned grid = (unsigned)(((unsigned long long)a->rows * groups + 7) / 8);
-    auto go = [&](auto* kernel) { return launch_pdl(kernel, dim3(grid), dim3(256), 0, st, k, steps, groups); };
+    const unsigned long long grid = ((unsigned long long)a->rows * groups + 7) / 8;
+    if (grid > 0x7fffffffu) return cudaErrorInvalidConfiguration;
+    auto go = [&](auto* kernel) { return launch_pdl(kernel, dim3((unsigned)grid), dim3(256), 0, st, k, steps, groups); };
     auto by_lanes = [&](auto half) {
         constexpr bool H = decltype(half)::value;
         return L == 2 ? go(qk_norm_rope_kernel<T, 2, H>) : L == 4 ? go(qk_norm_rope_kernel<T, 4, H>)

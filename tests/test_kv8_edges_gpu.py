@@ -1,6 +1,5 @@
-"""The 8-bit paged KV cache where its calls can go wrong: magnitudes at the ends of f32, streams that share a
-handle, row starts that do not describe the rows,
-positions outside the rotation table.
+"""The 8-bit paged KV cache where its calls can go wrong: magnitudes at the ends of f32, streams that share a handle,
+row starts that do not describe the rows, positions outside the rotation table, launches past the grid's limit.
 
 Stored bytes and scales follow the rule element by element in f32, so they are compared for equality with its numpy
 restatement (test_kv8_gpu.np_append)."""
@@ -228,3 +227,14 @@ def test_append_outside_the_rotation_table_leaves_the_page(be, dtype, rot, half,
                 half_page = slice(16 * 64 * side, 16 * 64 * (side + 1))
                 same = same and torch.equal(c.pages[b, :, half_page], before[b, :, half_page])
                 assert same == ((s, page) not in changed), (s, page, side)
+
+
+@pytest.mark.parametrize("rows,heads,hd", [(2 ** 26, 4096, 2), (2 ** 26, 513, 2), (2 ** 26, 2047, 512)])
+def test_norms_of_more_heads_than_a_launch_holds_are_refused(be, rows, heads, hd):
+    """(refused on the host: the sizes are the views' own, no memory of that size stands behind them)"""
+    x = torch.zeros(16, device="cuda", dtype=torch.half)
+    view = L.Rows(x.data_ptr(), L.POX_F16, heads * hd, hd)
+    args = L.QkNormRope(view, view, view, view, rows, heads, heads, hd, 0, 0, 1e-5, L.Rope(), 0)
+    with pytest.raises(L.PoxError):
+        be.qk_norm_rope(args, STREAM)
+    be.synchronize()
