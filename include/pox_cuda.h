@@ -373,7 +373,8 @@ int pox_cuda_qk_norm_rope(pox_cuda_ctx* ctx, const pox_qk_norm_rope* args, void*
  *   v of token t, dim d: byte 16 * hd + 16 * d + t
  * so that the attention's tensor-core operands are read from a page as it lies. head_dim 32, 64 or 128;
  * pages 16-byte, scales 8-byte aligned. Contents need no initialisation: a page counts as empty until
- * its slot 0 is written. */
+ * its slot 0 is written. A page filled by other means has scales that are not negative; to the attention a
+ * v scale below 1e-30 is 1e-30. */
 typedef struct {
     int8_t* pages;
     float* scales;

@@ -16,10 +16,10 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libpox_cuda.so")
 BUILD_DIR = os.path.join(PKG, "_build")
 
-SOURCES = ["pox_api.cu", "gemv.cu", "gemm_tc05.cu", "gemm_tcq.cu", "engine.cu", "comm.cu", "quantize.cu", "noalloc.cu", "persist.cu", "kv8.cu", "kv8_attn.cu", "kv8_prompt.cu",
-           "pox_file.cpp"]
-HEADERS = ["common.cuh", "gemv.cuh", "api_internal.h", "model.h", "comm.cuh", "tc05.cuh", "attn.cuh", "persist.h", "kv8.cuh",
-           "kv8_attn.h", "kv8_math.cuh"]
+SOURCES = ["pox_api.cu", "gemv.cu", "gemm_tc05.cu", "gemm_tcq.cu", "engine.cu", "comm.cu", "quantize.cu", "noalloc.cu",
+           "persist.cu", "kv8.cu", "kv8_attn.cu", "kv8_prompt.cu", "pox_file.cpp"]
+HEADERS = ["common.cuh", "gemv.cuh", "api_internal.h", "model.h", "comm.cuh", "tc05.cuh", "attn.cuh", "persist.h",
+           "kv8.cuh", "kv8_attn.h", "kv8_math.cuh"]
 
 
 def _nvcc() -> str:

@@ -280,8 +280,8 @@ enum { kTurnAny = 0, kTurnNone = 1, kTurnHalf = 2, kTurnPairs = 3 };
 // are that chain once or a few times.
 // A unit (page, kv head, side) is taken by two groups of HD / 4 lanes, lane c of group `hi` on dims 4 c .. 4 c + 3 of
 // tokens 8 hi .. 8 hi + 7, whose rows are all in flight at once (with all 16 tokens on a lane, 168 registers left 12
-// warps to an SM: no faster; a loop over the heads that fetches ahead: 66 us). The page's new rows set the scale, its older slots follow if the scale grew. A lane's four dims make a word of
-// each K row and 8 bytes of each of four V rows.
+// warps to an SM: no faster; a loop over the heads that fetches ahead: 66 us). The page's new rows set the scale, its
+// older slots follow if the scale grew. A lane's four dims make a word of each K row and 8 bytes of each of four V rows.
 template <int HD, typename T, int TURN>
 __global__ void __launch_bounds__(128, 5) kv8_append_kernel(AppendArgs<T> a, uint32_t ctas) {
     constexpr int L = HD / 4, UC = 128 / (2 * L), NT = kPage / 2;

@@ -277,8 +277,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
             tc_fence_after();
             const float inv = l == 0.f ? 0.f : 1.0f / l;
             const volatile uint32_t* place = place_s;
-        const int last_row = (int)place[0] + tid;
-        T* y = a.out.at((size_t)place[1] + (mine ? last_row / a.G : 0), h * a.G + (mine ? last_row % a.G : 0));
+            const int last_row = (int)place[0] + tid;
+            T* y = a.out.at((size_t)place[1] + (mine ? last_row / a.G : 0), h * a.G + (mine ? last_row % a.G : 0));
 #pragma unroll
             for (int c = 0; c < HD / 32; c++) {
                 float x[32];
@@ -384,51 +384,51 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8A
     } else {  // ---- the products: one thread of warp 12
         regs_less<kMmaRegs>();
         if (warp == 12 && lane == 0 && nk) {
-        constexpr uint32_t is = umma_idesc_f16(128, kPromptKeys), ip = umma_idesc_f16(128, HD);
-        auto wait_full = [&](int n) {
-            if (!bad) bad = !mbar_wait(full + 8 * (n % NST), (n / NST) & 1);
-            tc_fence_after();
-        };
-        auto release = [&](int n) {  // the stage, if the converters wait for it (nothing arrives there after the end)
-            if (n + NST < 2 * nk) umma_commit(empty + 8 * (n % NST));
-        };
-        auto scores = [&](int t, int j) {
-            const uint32_t k0 = kv + (2 * j % NST) * HB;
+            constexpr uint32_t is = umma_idesc_f16(128, kPromptKeys), ip = umma_idesc_f16(128, HD);
+            auto wait_full = [&](int n) {
+                if (!bad) bad = !mbar_wait(full + 8 * (n % NST), (n / NST) & 1);
+                tc_fence_after();
+            };
+            auto release = [&](int n) {  // the stage, if the converters wait for it (nothing arrives there after the end)
+                if (n + NST < 2 * nk) umma_commit(empty + 8 * (n % NST));
+            };
+            auto scores = [&](int t, int j) {
+                const uint32_t k0 = kv + (2 * j % NST) * HB;
 #pragma unroll
-            for (int k = 0; k < HD / 16; k++)
-                umma_f16(tm + TS + 128 * t, umma_desc_sw128(qs + t * QB + (k / 4) * (128 * 128)) + 2 * (k % 4),
-                         umma_desc_sw128(k0 + (k / 4) * (kPromptKeys * 128)) + 2 * (k % 4), is, k);
-            umma_commit(sfull + 8 * t);
-        };
-        auto values = [&](int t, int j) {
-            if (!bad) bad = !mbar_wait(pready + 8 * t, j & 1);
-            tc_fence_after();
-            if (bad) return;
-            const uint32_t v0 = kv + ((2 * j + 1) % NST) * HB;
+                for (int k = 0; k < HD / 16; k++)
+                    umma_f16(tm + TS + 128 * t, umma_desc_sw128(qs + t * QB + (k / 4) * (128 * 128)) + 2 * (k % 4),
+                             umma_desc_sw128(k0 + (k / 4) * (kPromptKeys * 128)) + 2 * (k % 4), is, k);
+                umma_commit(sfull + 8 * t);
+            };
+            auto values = [&](int t, int j) {
+                if (!bad) bad = !mbar_wait(pready + 8 * t, j & 1);
+                tc_fence_after();
+                if (bad) return;
+                const uint32_t v0 = kv + ((2 * j + 1) % NST) * HB;
 #pragma unroll
-            for (int k = 0; k < kPromptKeys / 16; k++)
-                umma_f16_ts(tm + TO + HD * t, tm + TS + 128 * t + 8 * k,
-                            umma_desc_sw128(v0 + (k / 4) * (HD * 128)) + 2 * (k % 4), ip, j || k);
-        };
-        wait_full(0);
-        if (!bad) {
-            for (int t = 0; t < nt; t++) scores(t, 0);
-            release(0);
-        }
-        for (int j = 0; j < nk && !bad; j++) {
-            wait_full(2 * j + 1);
-            for (int t = 0; t < nt && !bad; t++) {
-                values(t, j);
-                if (t == nt - 1) release(2 * j + 1);
-                if (j + 1 < nk) {
-                    if (t == 0) wait_full(2 * j + 2);
-                    if (!bad) scores(t, j + 1);
-                    if (t == nt - 1) release(2 * j + 2);
+                for (int k = 0; k < kPromptKeys / 16; k++)
+                    umma_f16_ts(tm + TO + HD * t, tm + TS + 128 * t + 8 * k,
+                                umma_desc_sw128(v0 + (k / 4) * (HD * 128)) + 2 * (k % 4), ip, j || k);
+            };
+            wait_full(0);
+            if (!bad) {
+                for (int t = 0; t < nt; t++) scores(t, 0);
+                release(0);
+            }
+            for (int j = 0; j < nk && !bad; j++) {
+                wait_full(2 * j + 1);
+                for (int t = 0; t < nt && !bad; t++) {
+                    values(t, j);
+                    if (t == nt - 1) release(2 * j + 1);
+                    if (j + 1 < nk) {
+                        if (t == 0) wait_full(2 * j + 2);
+                        if (!bad) scores(t, j + 1);
+                        if (t == nt - 1) release(2 * j + 2);
+                    }
                 }
             }
-        }
-        umma_commit(ofull);
-        if (bad) mbar_wait(ofull, 0);  // what was issued ends before the tensor memory is given back
+            umma_commit(ofull);
+            if (bad) mbar_wait(ofull, 0);  // what was issued ends before the tensor memory is given back
         }
     }
     if (bad && lane == 0) atomicOr(a.err, kErrWaitRing);
