@@ -624,8 +624,9 @@ static bool prompt_is_faster(const pox_kv8_cache* c, const pox_kv8_batch* b, int
 
 // The stream's places for the parts of items that a plan cuts, and their tickets: made by its first call, as large as any
 // plan on this device asks for, and not moved (a captured graph holds their addresses). Those of a stream that is
-// known to be destroyed go to the next new one, after a pox_cuda_synchronize and unless they were captured.
-static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, Kv8StepPlan& p) {
+// known to be destroyed go to the next new one, after a pox_cuda_synchronize and unless they were captured. A call that
+// does not use them (`used` false) makes them all the same, so that any first call readies the stream for a capture.
+static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, Kv8StepPlan& p, bool used) {
     try {
         std::lock_guard<std::mutex> lk(ctx->mu);
         auto same_handle = [&](const Kv8Scratch& x) {
@@ -635,6 +636,7 @@ static int kv8_scratch(pox_cuda_ctx* ctx, cudaStream_t st, Kv8StepPlan& p) {
         cudaError_t e = cudaStreamIsCapturing(st, &cs);
         if (e != cudaSuccess) return cuda_error(e, "stream of kv8_attention");
         if (cs != cudaStreamCaptureStatusNone) {  // (a stream's id is not to be had while it is captured)
+            if (!used) return POX_OK;
             for (auto& k : ctx->kv8)
                 if (same_handle(k.second) && k.second.tickets) {
                     k.second.captured = true;
@@ -890,7 +892,7 @@ extern "C" int pox_cuda_kv8_attention(pox_cuda_ctx* ctx, const pox_kv8_cache* c,
     Kv8StepPlan plan = kv8_step_plan(batch_view(b), (int)c->kv_heads, (int)c->head_dim, G, ctx->num_sms,
                                      prompt ? kPromptRows : 0x7fffffff);
     plan.device = ctx->device;
-    rc = step ? kv8_scratch(ctx, st, plan) : POX_OK;
+    rc = kv8_scratch(ctx, st, plan, step);
     if (rc) return rc;
     const int vec = vec4(q) && vec4(out);
     e = by_shape(c->head_dim, q->dtype, [&](auto hd, auto t) {

@@ -1,5 +1,6 @@
 """The 8-bit paged KV cache where its calls can go wrong: magnitudes at the ends of f32, streams that share a handle,
-row starts that do not describe the rows, positions outside the rotation table, launches past the grid's limit.
+row starts that do not describe the rows, positions outside the rotation table, launches past the grid's limit, first
+calls before a capture.
 
 Stored bytes and scales follow the rule element by element in f32, so they are compared for equality with its numpy
 restatement (test_kv8_gpu.np_append)."""
@@ -238,3 +239,31 @@ def test_norms_of_more_heads_than_a_launch_holds_are_refused(be, rows, heads, hd
     with pytest.raises(L.PoxError):
         be.qk_norm_rope(args, STREAM)
     be.synchronize()
+
+
+def test_any_first_call_readies_a_stream_for_capture(be):
+    """A prompt without the step kernel, then a captured decode step; and a captured prompt as a first call."""
+    c = Cache([1000], 8, 64, seed=1)
+    q = torch.randn(1000, 32, 64, device="cuda").bfloat16()
+    out, eager, last, want = (torch.empty_like(q[:n]) for n in (1000, 1000, 1, 1))
+    prompt, step = c.batch([0, 1000], [1000]), c.batch([0, 1], [1000])
+    be.kv8_attention(c.c, prompt, rows_of(q), rows_of(eager), 32, 0.0, STREAM)
+    be.kv8_attention(c.c, step, rows_of(q[999:]), rows_of(want), 32, 0.0, STREAM)
+    torch.cuda.synchronize()
+    st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    be.kv8_attention(c.c, prompt, rows_of(q), rows_of(out), 32, 0.0, st.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(out, eager)
+    with torch.cuda.graph(graph, stream=st):
+        be.kv8_attention(c.c, step, rows_of(q[999:]), rows_of(last), 32, 0.0, st.cuda_stream)
+    graph.replay()
+    be.synchronize()
+    assert torch.equal(last, want)
+    st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    out.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        be.kv8_attention(c.c, prompt, rows_of(q), rows_of(out), 32, 0.0, st.cuda_stream)
+    graph.replay()
+    be.synchronize()
+    assert torch.equal(out, eager)
