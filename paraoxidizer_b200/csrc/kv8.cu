@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(256, 3) qk_norm_rope_kernel(QkArgs<T> a, int s
     const uint32_t p = rot ? a.pos[r] : 0;
     if (rot && p >= a.rope.positions) {
         if (lane == 0) atomicOr(a.err, kErrRopePos);
+        asm volatile("cp.async.wait_all;" ::: "memory");  // the copies on their way end before the CTA does
         return;
     }
     // HALF: cosines and sines of the V pairs, two to a register pair. Else (cos, sin) and (-sin, cos) of each of them:

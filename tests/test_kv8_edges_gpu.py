@@ -230,6 +230,30 @@ def test_append_outside_the_rotation_table_leaves_the_page(be, dtype, rot, half,
                 assert same == ((s, page) not in changed), (s, page, side)
 
 
+@pytest.mark.parametrize("dtype,heads,hd", [("bf16", 64, 128), ("f32", 40, 64), ("f16", 9, 96)])
+def test_norms_at_positions_outside_the_table_leave_their_rows(be, dtype, heads, hd):
+    """Rows whose loads are on their way when the position is looked at; the rows around them are as without them."""
+    dt = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(500, heads, hd, generator=g, device="cuda").to(dt)
+    good, y = torch.zeros_like(x), torch.full_like(x, 7.0)
+    w = torch.ones(hd, device="cuda").half()
+    table = rope_table(600, hd)
+    pos = torch.arange(500, device="cuda", dtype=torch.int32)
+
+    def call(out, positions):
+        rope = L.Rope(table.data_ptr(), positions, hd, L.POX_ROPE_HALF)
+        be.qk_norm_rope(L.QkNormRope(rows_of(x), L.Rows(), rows_of(out), L.Rows(), 500, heads, 0, hd, w.data_ptr(), 0,
+                                     1e-5, rope, pos.data_ptr()), STREAM)
+
+    call(good, 600)
+    be.synchronize()
+    call(y, 333)
+    with pytest.raises(L.PoxError, match="rotation table"):
+        be.synchronize()
+    assert torch.equal(y[:333], good[:333]) and bool((y[333:] == 7.0).all())
+
+
 @pytest.mark.parametrize("rows,heads,hd", [(2 ** 26, 4096, 2), (2 ** 26, 513, 2), (2 ** 26, 2047, 512)])
 def test_norms_of_more_heads_than_a_launch_holds_are_refused(be, rows, heads, hd):
     """(refused on the host: the sizes are the views' own, no memory of that size stands behind them)"""
