@@ -418,9 +418,10 @@ int pox_cuda_kv8_read(pox_cuda_ctx* ctx, const pox_kv8_cache* cache, const pox_k
  *   out[r][h] = sum over t <= position(r) of p_t v_t, p = softmax_t(scale * q[r][h] . k_t)
  * for query head h over kv head h / (heads / kv_heads); scale 0 = 1 / sqrt(head_dim). Softmax statistics
  * and sums are f32; f16 and bf16 rows enter the products exactly, f32 rows as pairs of f16 (22
- * bits); a row that sees nothing is 0. q and out: rows [batch->rows][heads] of one dtype. Sequences of few
- * rows split their context over the GPU and are joined in the same launch, in a fixed order: results do
- * not change from run to run. out must not overlap q. The first call on a stream allocates that stream's
+ * bits); p is rounded to 22 bits for f32 rows and for f16 batches of at most 8 rows of a kv head to a
+ * sequence, else to 11; a row that sees nothing is 0. q and out: rows [batch->rows][heads] of one dtype.
+ * Sequences of few rows split their context over the GPU and are joined in the same launch, in a fixed
+ * order: results do not change from run to run. out must not overlap q. The first call on a stream allocates that stream's
  * split partials (about 5 MB, held by the context, enough for all later calls): make it before capturing
  * the stream. A captured call keeps to the partials of the stream that it was captured on, so its replays
  * must not run beside other calls on that stream. Streams are told apart by identity, not by handle:

@@ -612,8 +612,8 @@ constexpr int kPromptRows = 64;
 // kernel spreads rows by 16 and the context over the whole GPU, a page of a tile at about 0.65 ns (head dim 128; 64:
 // 0.46); a CTA of the prompt kernel walks the context for 256 rows, 128 tokens in 2.75 us (up to 128 rows 2.35; head dim
 // 64: 2.35 and 2.05). Both ways measured, bf16, 8 kv heads of 128 with 4 query heads each, step against prompt kernel:
-// one sequence of 128 rows at 4096 tokens 59 us against 90, of 512 at 512 43 against 31; eight of 32 rows at 4096 103
-// against 77, of 16 61 against 75; one of 256 at 32768 580 against 556.
+// one sequence of 128 rows at 4096 tokens 61 us against 87, of 512 at 512 43 against 30; eight of 32 rows at 4096 108
+// against 77, of 16 61 against 63; one of 256 at 32768 626 against 544.
 static bool prompt_is_faster(const pox_kv8_cache* c, const pox_kv8_batch* b, int G, int sms) {
     const double rows = (double)b->rows * G, most = (double)std::min(b->max_rows, b->rows) * G;
     const bool wide = c->head_dim == 128;

@@ -70,9 +70,9 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 // rounding remains), one for bf16 and for more rows (2^-11 of p).
 //
 // What bounds it: HBM where the contexts are long (64 sequences of 3800 to 4400 tokens, 64 heads over 8 of 128, bf16:
-// 541 MB in 97 us, 85 % of the measured copy rate; the three above 106 us, 83 %); the start and joining of items
-// where there are many short ones (37 sequences of up to 2011 tokens, 12 heads of 64: 24 us, its bytes 8.4); for f32
-// rows the products of two terms each (20 prompts of up to 257 rows, 14 heads over 2 of 64: 127 us, mma.sync pipe 40 %
+// 541 MB in 97 us, 85 % of the measured copy rate; the three above 109 us, 81 %); the start and joining of items
+// where there are many short ones (37 sequences of up to 2011 tokens, 12 heads of 64: 25 us, its bytes 8.4); for f32
+// rows the products of two terms each (20 prompts of up to 257 rows, 14 heads over 2 of 64: 128 us, mma.sync pipe 40 %
 // and issue slots 45 % busy at the 8 warps that the registers leave an SM); one sequence of 640 tokens the launch (5.6).
 constexpr uint32_t kWholePages = 128;
 
