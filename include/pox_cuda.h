@@ -421,13 +421,13 @@ int pox_cuda_kv8_read(pox_cuda_ctx* ctx, const pox_kv8_cache* cache, const pox_k
  * bits); p is rounded to 22 bits for f32 rows and for f16 batches of at most 8 rows of a kv head to a
  * sequence, else to 11; a row that sees nothing is 0. q and out: rows [batch->rows][heads] of one dtype.
  * Sequences of few rows split their context over the GPU and are joined in the same launch, in a fixed
- * order: results do not change from run to run. out must not overlap q. The first call on a stream allocates that stream's
- * split partials (about 5 MB, held by the context, enough for all later calls): make it before capturing
- * the stream. A captured call keeps to the partials of the stream that it was captured on, so its replays
- * must not run beside other calls on that stream. Streams are told apart by identity, not by handle:
- * cudaStreamPerThread has partials for each thread, and a new stream that is given a destroyed one's handle
- * does not share them while that one's work may run (they go to a new stream after the next
- * pox_cuda_synchronize, unless a graph holds them). A sequence has at most 2^30 rows times query heads of a
+ * order: results do not change from run to run. out must not overlap q. The first call on a stream
+ * allocates that stream's split partials (about 5 MB, held by the context, enough for all later calls):
+ * make it before capturing the stream. A captured call keeps to the partials of the stream that it was
+ * captured on, so its replays must not run beside other calls on that stream. Streams are told apart by
+ * identity, not by handle: cudaStreamPerThread has partials for each thread, and a new stream that is given
+ * a destroyed one's handle does not share them while that one's work may run (they go to a new stream after
+ * the next pox_cuda_synchronize, unless a graph holds them). A sequence has at most 2^30 rows times query heads of a
  * kv head (else POX_ERR_UNSUPPORTED). A batch of sequences whose pages, counted once for each 16 such rows
  * and kv head, sum to about 2^32 is refused on the device (POX_ERR_INVALID from the next
  * pox_cuda_synchronize; f16 and bf16 prompts of head_dim 64 and 128 that are worth a CTA of their own do

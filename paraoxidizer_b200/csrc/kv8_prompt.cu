@@ -94,8 +94,9 @@ struct PromptSmem {
 // O stays in TMEM through the context, where each product cuts off what it adds to: 1.1e-9 of an output for each token
 // seen, 1.3e-4 at 131072, below the roundings of f16 and of p.
 // 8192 rows over themselves, 32 heads over 8 of 128, bf16: 657 to 670 us (632 on one box of six), 820 to 870 TFLOP/s, 50
-// to 53 % of the measured rate of library products. The round trip of a tile bounds it: a row tile's next product waits for its softmax, and the
-// two softmaxes together take longer than the products that they hide (tensor pipe 40 % busy, exponentials 41 %).
+// to 53 % of the measured rate of library products. The round trip of a tile bounds it: a row tile's next product waits
+// for its softmax, and the two softmaxes together take longer than the products that they hide (tensor pipe 40 % busy,
+// exponentials 41 %).
 // An MMA completes in order with those issued before it: S of tile j ready means P V of tile j - 1 done.
 template <int HD, typename T>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv8_attn_prompt_kernel(Kv8Attn<T> a, int min_rows) {
